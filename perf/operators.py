@@ -1,0 +1,370 @@
+"""Workloads of the sequence-encoder and training operators: a gated linear recurrence with its scan over time, a gated
+feed-forward product, and the global gradient norm with the clipped optimizer step that consumes it.
+
+``run`` computes an operator in its plain form (elementary torch operations, 32 bits, one rounding at the end) or, with
+``own`` set, through this package's public entry points; ``exact`` gives the same outputs from the definition in 64 bits.
+"""
+import math
+
+import torch
+
+own = False
+
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+EPS_CLIP = 1e-6
+
+
+def listed():
+    return [
+        # One new token of 32 streams that are being answered at once: the state goes in and comes out, latency is all that counts.
+        dict(name="scan_token", op="scan", dtype="bf16", train=False, B=32, L=1, D=1024, ragged=False, joined=True, state=True),
+        # The 51-point load history of the U-Net's conditioning at its width of 256, a training batch of four, in the model's fp32.
+        dict(name="scan_signal", op="scan", dtype="f32", train=True, B=4, L=51, D=256, ragged=False, joined=True, state=False),
+        # One very long recording in one piece: few channels times sequences, so the time axis itself has to be split.
+        dict(name="scan_long", op="scan", dtype="bf16", train=False, B=1, L=65536, D=1024, ragged=False, joined=False, state=True),
+        # A training batch of recordings of unequal length, padded to the longest, an odd length and width.
+        dict(name="scan_train", op="scan", dtype="bf16", train=True, B=8, L=4093, D=1000, ragged=True, joined=True, state=False),
+        # A few rows at a time through wide weights: answering, bound by reading the weights.
+        dict(name="ff_token", op="ff", dtype="bf16", train=False, M=4, K=1024, F=4096, act="silu", bias=False),
+        # The tokens of four load histories (4 x 51 rows) in the U-Net's conditioning width, with the gradients, in fp32.
+        dict(name="ff_signal", op="ff", dtype="f32", train=True, M=204, K=256, F=512, act="silu", bias=True),
+        # Many rows through large weights, no gradients: the throughput case.
+        dict(name="ff_rows", op="ff", dtype="bf16", train=False, M=8192, K=2048, F=8192, act="silu", bias=False),
+        # A training step on a batch whose sizes fit no tile, in the fp16 of the mixed-precision recipe.
+        dict(name="ff_train", op="ff", dtype="f16", train=True, M=3996, K=1000, F=4096, act="gelu", bias=True),
+        # The norm that a training loop logs and clips by: the gradients of a U-Net-sized model, a few hundred tensors.
+        dict(name="norm_model", op="norm", dtype="f32", tensors=367, total=39_500_000),
+        # The same over gradients kept in bf16, of a larger model.
+        dict(name="norm_large", op="norm", dtype="bf16", tensors=240, total=400_000_000),
+        # The clipped optimizer step of a small encoder alone: few small tensors, launches are what it costs.
+        dict(name="adam_small", op="adam", dtype="f32", tensors=18, total=1_300_000),
+        # The clipped optimizer step of the U-Net-sized model.
+        dict(name="adam_model", op="adam", dtype="f32", tensors=367, total=39_500_000),
+    ]
+
+
+def _log(rng, low, high):
+    return max(low, min(high, int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))))
+
+
+def draw(rng):
+    op = rng.choice(["scan", "scan", "ff", "ff", "norm", "adam"])
+    dtype = rng.choice(["f32", "bf16", "f16"])
+    if op == "scan":
+        train = rng.random() < 0.5
+        B, D = _log(rng, 1, 48), _log(rng, 5, 2500)
+        L = _log(rng, 1, max(2, min(65536, 24_000_000 // (B * D))))
+        return dict(op=op, dtype=dtype, train=train, B=B, L=L, D=D, ragged=rng.random() < 0.4, joined=rng.random() < 0.5, state=rng.random() < 0.5)
+    if op == "ff":
+        train = rng.random() < 0.5
+        K, F = _log(rng, 24, 2048), _log(rng, 40, 8192)
+        if rng.random() < 0.6:  # widths are mostly round numbers, rows hardly ever
+            K, F = (K + 7) // 8 * 8, (F + 7) // 8 * 8
+        M = _log(rng, 1, min(8192, 40_000_000_000 // (K * F)))
+        return dict(op=op, dtype=dtype, train=train, M=M, K=K, F=F, act=rng.choice(["silu", "gelu"]), bias=rng.random() < 0.5)
+    n = _log(rng, 1, 400)
+    return dict(op=op, dtype=dtype, tensors=n, total=n * 3 + _log(rng, 2_000, 30_000_000))
+
+
+def _sizes(case):
+    """Element counts of a model's parameter tensors: from a few values (norms, biases) to the large matrices, over their logarithm."""
+    n, total = case["tensors"], case["total"]
+    raw = [math.exp(9.0 * ((i * 0.6180339887) % 1.0)) for i in range(n)]
+    unit = total / sum(raw)
+    sizes = [max(1, int(unit * r)) for r in raw]
+    sizes[0] += max(0, total - sum(sizes))
+    return sizes
+
+
+def _views(flat, sizes):
+    starts = [0]
+    for n in sizes:
+        starts.append(starts[-1] + (n + 3) // 4 * 4)
+    return [flat[o:o + n] for o, n in zip(starts, sizes)]
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    dt = DTYPES[case["dtype"]]
+
+    def normal(*shape, scale=1.0, dtype=dt):
+        return torch.randn(*shape, generator=gen, device="cuda", dtype=torch.float32).mul_(scale).to(dtype)
+
+    state = dict(case)
+    if case["op"] == "scan":
+        B, L, D = case["B"], case["L"], case["D"]
+        # forget gates from a memory of two steps to one of a few thousand, as such layers are initialised, one per channel
+        lean = torch.linspace(0.0, 8.0, D, device="cuda")[torch.randperm(D, generator=gen, device="cuda")]
+        both = torch.empty(B, L, 2 * D, device="cuda", dtype=dt)
+        both[..., :D] = normal(B, L, D)
+        both[..., D:] = (torch.randn(B, L, D, generator=gen, device="cuda") + lean).to(dt)
+        # candidates and gates are the two halves of one projection's rows, or tensors of their own
+        x, gate = (both[..., :D], both[..., D:]) if case["joined"] else (both[..., :D].contiguous(), both[..., D:].contiguous())
+        state["x"], state["gate"] = x.detach(), gate.detach()
+        state["h0"] = normal(B, D, dtype=torch.float32) if case["state"] else None
+        state["lengths"] = torch.randint((L + 1) // 2, L + 1, (B,), generator=gen, device="cuda", dtype=torch.int32) if case["ragged"] else None
+        if case["train"]:
+            state["dy"], state["dlast"] = normal(B, L, D), normal(B, D, dtype=torch.float32)
+            for k in ("x", "gate", "h0"):
+                if state[k] is not None:
+                    state[k].requires_grad_(True)
+    elif case["op"] == "ff":
+        M, K, F = case["M"], case["K"], case["F"]
+        state["x"] = normal(M, K)
+        state["wg"], state["wu"] = normal(F, K, scale=K ** -0.5), normal(F, K, scale=K ** -0.5)
+        state["bg"], state["bu"] = (normal(F, scale=0.1), normal(F, scale=0.1)) if case["bias"] else (None, None)
+        if case["train"]:
+            state["dh"] = normal(M, F)
+            for k in ("x", "wg", "wu", "bg", "bu"):
+                if state[k] is not None:
+                    state[k].requires_grad_(True)
+    else:
+        sizes = _sizes(case)
+        state["grads"] = [normal(n, scale=0.02) for n in sizes]
+        if case["op"] == "adam":
+            # weights and moments live in one buffer each, every tensor's start a multiple of four values
+            room = sum((n + 3) // 4 * 4 for n in sizes)
+            flat = [normal(room, scale=0.05, dtype=torch.float32), normal(room, scale=1e-3, dtype=torch.float32),
+                    normal(room, scale=1e-3, dtype=torch.float32).square_()]
+            state["flat"] = flat
+            state["params"], state["m"], state["v"] = (_views(f, sizes) for f in flat)
+            state["step"] = 100
+    return state
+
+
+# ---- plain forms
+
+
+def _doubling(f, b, h0):
+    """h_t = f_t h_(t-1) + b_t over dim 1 by pairwise doubling of the maps h -> f h + b."""
+    b = torch.cat([b[:, :1] + f[:, :1] * h0[:, None], b[:, 1:]], 1)
+    L, d = b.shape[1], 1
+    while d < L:
+        b = torch.cat([b[:, :d], torch.addcmul(b[:, d:], f[:, d:], b[:, :-d])], 1)
+        f = torch.cat([f[:, :d], f[:, d:] * f[:, :-d]], 1)
+        d *= 2
+    return b
+
+
+def _plain_scan(s):
+    x, g = s["x"].detach(), s["gate"].detach()
+    dt, (B, L, D) = x.dtype, x.shape
+    x, g = x.float(), g.float()
+    h0 = torch.zeros(B, D, device=x.device) if s["h0"] is None else s["h0"].detach()
+    f, i = 1 / (1 + torch.exp(-g)), 1 / (1 + torch.exp(g))
+    if s["lengths"] is not None:  # behind a sequence's end the state stands still
+        live = (torch.arange(L, device=x.device)[None, :] < s["lengths"][:, None])[..., None]
+        f, i, x = torch.where(live, f, 1.0), torch.where(live, i, 0.0), torch.where(live, x, 0.0)
+    h = _doubling(f, i * x, h0)
+    last = h[:, -1].clone()
+    y = (h if s["lengths"] is None else torch.where(live, h, 0.0)).to(dt)
+    if not s["train"]:
+        return y, last
+    dy = s["dy"].float()
+    if s["lengths"] is not None:
+        dy = torch.where(live, dy, 0.0)
+    # dh_t = dy_t + f_(t+1) dh_(t+1), the last step's with the final state's gradient
+    dy = torch.cat([dy[:, :-1], dy[:, -1:] + s["dlast"][:, None]], 1)
+    back = torch.cat([torch.zeros_like(f[:, :1]), f[:, 1:].flip(1)], 1)
+    dh = _doubling(back, dy.flip(1), torch.zeros_like(h0)).flip(1)
+    before = torch.cat([h0[:, None], h[:, :-1]], 1)
+    dx, dg = dh * i, dh * (before - x) * f * i
+    out = [y, last, dx.to(dt), dg.to(dt)]
+    if s["h0"] is not None:
+        out.append(f[:, 0] * dh[:, 0])
+    return tuple(out)
+
+
+def _act(g, act):
+    """The activation and its derivative."""
+    if act == "silu":
+        p = 1 / (1 + torch.exp(-g))
+        return g * p, p * (1 + g * (1 - p))
+    p = 0.5 * (1 + torch.erf(g * math.sqrt(0.5)))
+    return g * p, p + g * torch.exp(-0.5 * g * g) * (1 / math.sqrt(2 * math.pi))
+
+
+def _feed_forward(s, wide):
+    """Outputs and gradients with every product in the type `wide`."""
+    x, wg, wu = (s[k].detach().to(wide) for k in ("x", "wg", "wu"))
+    g, u = x @ wg.t(), x @ wu.t()
+    if s["bg"] is not None:
+        g, u = g + s["bg"].detach().to(wide), u + s["bu"].detach().to(wide)
+    a, slope = _act(g, s["act"])
+    h = a * u
+    if not s["train"]:
+        return [h]
+    dh = s["dh"].to(wide)
+    dg, du = dh * u * slope, dh * a
+    out = [h, dg @ wg + du @ wu, dg.t().contiguous() @ x, du.t().contiguous() @ x]
+    if s["bg"] is not None:
+        out += [dg.sum(0), du.sum(0)]
+    return out
+
+
+def _plain_ff(s):
+    return tuple(t.to(s["x"].dtype) for t in _feed_forward(s, torch.float32))
+
+
+def _adam_scalars(s):
+    return dict(lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, max_norm=1.0, step=s["step"])
+
+
+def _plain_norm(grads):
+    # 64 bits for the sum over all of the model's values
+    return torch.stack([g.float().double().square().sum() for g in grads]).sum().sqrt()
+
+
+def _plain_adam(s):
+    k = _adam_scalars(s)
+    s["step"] += 1  # the next pass is the next step
+    norm = _plain_norm(s["grads"])
+    coef = torch.clamp(k["max_norm"] / (norm + EPS_CLIP), max=1.0).float()
+    c1, c2 = 1 - k["b1"] ** k["step"], math.sqrt(1 - k["b2"] ** k["step"])
+
+    def one(p, g, m, v):
+        g = g.float() * coef
+        m.mul_(k["b1"]).add_(g * (1 - k["b1"]))
+        v.mul_(k["b2"]).add_(g * g * (1 - k["b2"]))
+        p.sub_(m / (v.sqrt() / c2 + k["eps"]) * (k["lr"] / c1))
+
+    [one(*t) for t in zip(s["params"], s["grads"], s["m"], s["v"])]
+    return (norm.float(), *s["flat"])
+
+
+# ---- the framework's own operators
+
+
+def _own_scan(s):
+    from videometamaterials_amd import gated_linear_scan
+    y, last = gated_linear_scan(s["x"], s["gate"], h0=s["h0"], lengths=s["lengths"])
+    if not s["train"]:
+        return y, last
+    leaves = [s[k] for k in ("x", "gate", "h0") if s[k] is not None]
+    return (y.detach(), last.detach()) + torch.autograd.grad((y, last), leaves, (s["dy"], s["dlast"]))
+
+
+def _own_ff(s):
+    from videometamaterials_amd import gated_feed_forward
+    h = gated_feed_forward(s["x"], s["wg"], s["wu"], s["bg"], s["bu"], activation=s["act"])
+    if not s["train"]:
+        return (h,)
+    leaves = [s[k] for k in ("x", "wg", "wu", "bg", "bu") if s[k] is not None]
+    return (h.detach(),) + torch.autograd.grad(h, leaves, s["dh"])
+
+
+def _own_norm(s):
+    from videometamaterials_amd import grad_norm
+    return grad_norm(s["grads"])
+
+
+def _own_adam(s):
+    from videometamaterials_amd import clipped_adam_step_
+    k = _adam_scalars(s)
+    s["step"] += 1
+    norm = clipped_adam_step_(s["params"], s["grads"], s["m"], s["v"], step=k["step"], lr=k["lr"], betas=(k["b1"], k["b2"]), eps=k["eps"],
+                              max_norm=k["max_norm"])
+    return (norm, *s["flat"])
+
+
+def run(state):
+    if own:
+        return {"scan": _own_scan, "ff": _own_ff, "norm": _own_norm, "adam": _own_adam}[state["op"]](state)
+    if state["op"] == "norm":
+        return _plain_norm(state["grads"]).float()
+    return {"scan": _plain_scan, "ff": _plain_ff, "adam": _plain_adam}[state["op"]](state)
+
+
+def work(case):
+    size = 4 if case["dtype"] == "f32" else 2
+    if case["op"] == "scan":
+        n = case["B"] * case["L"] * case["D"]
+        live = 0.75 if case["ragged"] else 1.0  # lengths are uniform between half and all of L: rows behind the end are written, not read
+        if case["train"]:
+            return {"bytes": int(n * size * (3 * live + 3)), "flops": int(25 * n * live)}
+        return {"bytes": int(n * size * (2 * live + 1)), "flops": int(8 * n * live)}
+    if case["op"] == "ff":
+        M, K, F = case["M"], case["K"], case["F"]
+        if case["train"]:
+            return {"bytes": size * (2 * M * K + 4 * F * K + 2 * M * F), "flops": 12 * M * K * F}
+        return {"bytes": size * (M * K + 2 * F * K + M * F), "flops": 4 * M * K * F}
+    if case["op"] == "norm":
+        return {"bytes": case["total"] * size, "flops": 2 * case["total"]}
+    return {"bytes": case["total"] * (24 + size), "flops": 16 * case["total"]}
+
+
+# ---- the definitions in 64 bits
+
+
+def _steps(f, b, h):
+    """h_t = f_t h_(t-1) + b_t step by step, side by side in equal pieces of the time axis, which are then joined in order."""
+    B, L, D = f.shape
+    c = max(1, math.isqrt(L))
+    n = -(-L // c)
+    pad = n * c - L
+    f = torch.cat([f, torch.ones(B, pad, D, dtype=f.dtype, device=f.device)], 1).view(B, n, c, D)
+    b = torch.cat([b, torch.zeros(B, pad, D, dtype=b.dtype, device=b.device)], 1).view(B, n, c, D)
+    through, own_part = torch.empty_like(f), torch.empty_like(b)
+    p, q = torch.ones_like(f[:, :, 0]), torch.zeros_like(b[:, :, 0])
+    for t in range(c):
+        p, q = p * f[:, :, t], q * f[:, :, t] + b[:, :, t]
+        through[:, :, t], own_part[:, :, t] = p, q
+    for k in range(n):
+        own_part[:, k] += through[:, k] * h[:, None]
+        h = own_part[:, k, -1]
+    return own_part.view(B, n * c, D)[:, :L]
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    with torch.no_grad():
+        if case["op"] == "scan":
+            x, g = s["x"].double(), s["gate"].double()
+            B, L, D = x.shape
+            keep, take = torch.sigmoid(g), torch.sigmoid(-g)
+            h0 = torch.zeros(B, D, dtype=torch.float64, device="cuda") if s["h0"] is None else s["h0"].double()
+            at = torch.arange(L, device="cuda").view(1, L, 1)
+            end = torch.full((B, 1, 1), L, device="cuda") if s["lengths"] is None else s["lengths"].long().view(B, 1, 1)
+            behind = (at >= end).expand(B, L, D)
+            keep, take, x = keep.masked_fill(behind, 1.0), take.masked_fill(behind, 0.0), x.masked_fill(behind, 0.0)
+            h = _steps(keep, take * x, h0)
+            out = [h.masked_fill(behind, 0.0), h[:, -1].clone()]
+            if case["train"]:
+                dy = s["dy"].double().masked_fill(behind, 0.0)
+                # c_t = f_t (dy_t + c_(t+1)): what a step hands to the one before it
+                c = _steps(keep.flip(1), (keep * dy).flip(1), s["dlast"].double()).flip(1)
+                dh = dy + torch.cat([c[:, 1:], s["dlast"].double()[:, None]], 1)
+                out += [dh * take, dh * (torch.cat([h0[:, None], h[:, :-1]], 1) - x) * keep * take]
+                if s["h0"] is not None:
+                    out.append(c[:, 0].clone())
+            return tuple(out)
+        if case["op"] == "ff":
+            x, wg, wu = s["x"].double(), s["wg"].double(), s["wu"].double()
+            g, u = torch.nn.functional.linear(x, wg), torch.nn.functional.linear(x, wu)
+            if s["bg"] is not None:
+                g, u = g + s["bg"].double(), u + s["bu"].double()
+            if case["act"] == "silu":
+                a, slope = g * torch.sigmoid(g), torch.sigmoid(g) * (1 + g * torch.sigmoid(-g))
+            else:
+                cdf = torch.special.ndtr(g)
+                a, slope = g * cdf, cdf + g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+            if not case["train"]:
+                return (a * u,)
+            dg, du = s["dh"].double() * u * slope, s["dh"].double() * a
+            out = [a * u, torch.mm(dg, wg) + torch.mm(du, wu), torch.mm(dg.t(), x), torch.mm(du.t(), x)]
+            if s["bg"] is not None:
+                out += [dg.sum(0), du.sum(0)]
+            return tuple(out)
+        norm = torch.linalg.vector_norm(torch.stack([torch.linalg.vector_norm(g.double()) for g in s["grads"]]))
+        if case["op"] == "norm":
+            return norm
+        k = _adam_scalars(s)
+        coef = min(1.0, k["max_norm"] / (norm.item() + EPS_CLIP))
+        flat = [f.double() for f in s["flat"]]
+        for p, g, m, v in zip(*(_views(f, _sizes(case)) for f in flat[:1]), s["grads"], *(_views(f, _sizes(case)) for f in flat[1:])):
+            g = g.double() * coef
+            m.copy_(k["b1"] * m + (1 - k["b1"]) * g)
+            v.copy_(k["b2"] * v + (1 - k["b2"]) * g ** 2)
+            mean, var = m / (1 - k["b1"] ** k["step"]), v / (1 - k["b2"] ** k["step"])
+            p.copy_(p - k["lr"] * mean / (var.sqrt() + k["eps"]))
+        return (norm, *flat)
