@@ -259,11 +259,12 @@ def _own_norm(s):
 
 
 def _own_adam(s):
-    from videometamaterials_amd import clipped_adam_step_
+    from videometamaterials_amd import ClippedAdam
     k = _adam_scalars(s)
-    s["step"] += 1
-    norm = clipped_adam_step_(s["params"], s["grads"], s["m"], s["v"], step=k["step"], lr=k["lr"], betas=(k["b1"], k["b2"]), eps=k["eps"],
-                              max_norm=k["max_norm"])
+    if "optimizer" not in s:  # a training program makes its optimizer once
+        s["optimizer"] = ClippedAdam(s["params"], exp_avgs=s["m"], exp_avg_sqs=s["v"], step=k["step"] - 1, lr=k["lr"], betas=(k["b1"], k["b2"]),
+                                     eps=k["eps"], max_norm=k["max_norm"])
+    norm = s["optimizer"].step(s["grads"])
     return (norm, *s["flat"])
 
 
