@@ -36,7 +36,10 @@ SINGLE_PASS_SOURCES = {"temporal_block_bwd.hip", "linattn_block_bwd.hip", "qkv_b
 #   matrix pipe (55 % for the scalar forms; MI355X_MICROARCH.md "price of one filler beside MFMAs", LABNOTES 7.6).  Measured on one box, libraries
 #   alternating (LABNOTES 10.2): captured sampling step 13.31 -> 13.08 ms, training step 33.97 -> 33.75 ms; it also removes the compiler-made packed
 #   sequences of the kind LABNOTES 9.8 suspected behind the rotated-token-key corruption (the hand-written v_pk intrinsics stay).
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=on", "-munsafe-fp-atomics", "-fno-slp-vectorize"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 at all -- vector types and intrinsics make them too, and some of their forms have given wrong results now
+#   and then (the host pass of hipcc does not know the feature and says so; harmless)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=on", "-munsafe-fp-atomics", "-fno-slp-vectorize",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 if EXPERIMENTS:
     FLAGS.append("-DVMM_EXPERIMENTS=1")
 
