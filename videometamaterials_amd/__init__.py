@@ -9,5 +9,8 @@ from .diffusion import GaussianDiffusion  # noqa: F401
 from . import hostmath  # noqa: F401
 from .geometry import extract_geometries  # noqa: F401
 from .dataset import Dataset  # noqa: F401
+from .sequence import gated_linear_scan, gated_feed_forward  # noqa: F401
+from .optim import ClippedAdam, clip_grad_norm_, grad_norm  # noqa: F401
 
-__all__ = ["Unet3D", "GaussianDiffusion", "hostmath", "extract_geometries", "Dataset"]
+__all__ = ["Unet3D", "GaussianDiffusion", "hostmath", "extract_geometries", "Dataset", "gated_linear_scan", "gated_feed_forward", "ClippedAdam",
+           "clip_grad_norm_", "grad_norm"]

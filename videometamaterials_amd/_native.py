@@ -111,6 +111,53 @@ class OptimJob(C.Structure):
     _fields_ = [("p", c_ptr), ("g", c_ptr), ("m", c_ptr), ("v", c_ptr), ("n", c_i64)]
 
 
+class GatedScanDesc(C.Structure):
+    """vmm_gated_scan_desc (include/vmm_kernels.h)."""
+
+    _fields_ = [
+        ("x", c_ptr), ("x_batch", c_i64), ("x_row", c_i64),
+        ("gate", c_ptr), ("gate_batch", c_i64), ("gate_row", c_i64),
+        ("y", c_ptr), ("y_batch", c_i64), ("y_row", c_i64),
+        ("h0", c_ptr), ("h_last", c_ptr), ("lengths", c_ptr), ("states", c_ptr),
+        ("dy", c_ptr), ("dy_batch", c_i64), ("dy_row", c_i64),
+        ("dx", c_ptr), ("dx_batch", c_i64), ("dx_row", c_i64),
+        ("dgate", c_ptr), ("dgate_batch", c_i64), ("dgate_row", c_i64),
+        ("dh_last", c_ptr), ("dh0", c_ptr),
+        ("workspace", c_ptr),
+        ("L", c_i64),
+        ("B", c_i32), ("D", c_i32), ("type", c_i32),
+    ]
+
+
+class GatedFFDesc(C.Structure):
+    """vmm_gated_ff_desc (include/vmm_kernels.h)."""
+
+    _fields_ = [
+        ("x", c_ptr), ("ldx", c_i64),
+        ("w_gate", c_ptr), ("w_up", c_ptr), ("b_gate", c_ptr), ("b_up", c_ptr),
+        ("h", c_ptr), ("ldh", c_i64),
+        ("g_pre", c_ptr), ("u_pre", c_ptr),
+        ("dh", c_ptr), ("lddh", c_i64),
+        ("dx", c_ptr), ("lddx", c_i64),
+        ("dw_gate", c_ptr), ("dw_up", c_ptr), ("db_gate", c_ptr), ("db_up", c_ptr),
+        ("workspace", c_ptr),
+        ("M", c_i64),
+        ("K", c_i32), ("F", c_i32), ("type", c_i32), ("act", c_i32),
+    ]
+
+
+class GradJob(C.Structure):
+    """vmm_grad_job (include/vmm_kernels.h)."""
+
+    _fields_ = [("g", c_ptr), ("n", c_i64), ("type", c_i32), ("reserved", c_i32)]
+
+
+class ClipAdamJob(C.Structure):
+    """vmm_clip_adam_job (include/vmm_kernels.h)."""
+
+    _fields_ = [("p", c_ptr), ("g", c_ptr), ("m", c_ptr), ("v", c_ptr), ("n", c_i64), ("type", c_i32), ("reserved", c_i32)]
+
+
 # name -> argtypes (restype is always int); must list EVERY symbol include/vmm_kernels.h declares
 SIGNATURES = {
     "vmm_conv_igemm_f32": [C.POINTER(ConvDesc), c_ptr],
@@ -291,6 +338,18 @@ SIGNATURES = {
     "vmm_loss_reduce": [c_ptr, c_ptr, c_i64, c_i32, c_ptr, c_ptr, c_ptr],
     "vmm_cfg_combine": [c_ptr, c_ptr, c_f32, c_ptr, c_i64, c_ptr],
     "vmm_lincomb": [c_ptr, c_ptr, c_ptr, c_f32, c_f32, c_f32, c_f32, c_ptr, c_i64, c_ptr],
+    # operators of sequence encoders and of their training
+    "vmm_gated_scan_states": [C.POINTER(GatedScanDesc)],
+    "vmm_gated_scan_workspace": [C.POINTER(GatedScanDesc), c_i32],
+    "vmm_gated_scan": [C.POINTER(GatedScanDesc), c_ptr],
+    "vmm_gated_scan_bwd": [C.POINTER(GatedScanDesc), c_ptr],
+    "vmm_gated_ff_workspace": [C.POINTER(GatedFFDesc), c_i32],
+    "vmm_gated_ff": [C.POINTER(GatedFFDesc), c_ptr],
+    "vmm_gated_ff_bwd": [C.POINTER(GatedFFDesc), c_ptr],
+    "vmm_grad_norm_workspace": [c_ptr, c_i32],
+    "vmm_grad_norm": [c_ptr, c_i32, c_f32, c_f32, c_ptr, c_ptr, c_ptr, c_ptr],
+    "vmm_grad_clip": [c_ptr, c_i32, c_ptr, c_ptr],
+    "vmm_adam_step_clipped": [c_ptr, c_i32, C.c_double, C.c_double, C.c_double, C.c_double, c_i64, c_f32, c_ptr, c_ptr, c_ptr],
 }
 
 # include/vmm_experiments.h: entry points of libvmm_hip_exp.so only (VMM_EXPERIMENTS=1 build; bound when the loaded library exports them)
@@ -326,7 +385,7 @@ DP_SIGNATURES = {
     "vmm_dp_finalize": [c_ptr],
 }
 
-RESTYPES = {"vmm_dp_last_error": C.c_char_p, "vmm_attention_bwd_scratch": c_i64, "vmm_cross_attention_bwd_scratch": c_i64, "vmm_linattn_block_workspace": c_i64, "vmm_conv3x3_wgrad_bf16x3_workspace": c_i64, "vmm_conv1x1_wgrad_bf16x3_workspace": c_i64, "vmm_conv_wgrad_tap_workspace": c_i64, "vmm_qkv_bwd_workspace": c_i64, "vmm_temporal_block_bwd_workspace": c_i64, "vmm_linattn_block_bwd_workspace": c_i64, "vmm_groupnorm_bwd_scratch": c_i64}  # everything else returns int (0 = ok)
+RESTYPES = {"vmm_gated_scan_states": c_i64, "vmm_gated_scan_workspace": c_i64, "vmm_gated_ff_workspace": c_i64, "vmm_grad_norm_workspace": c_i64, "vmm_dp_last_error": C.c_char_p, "vmm_attention_bwd_scratch": c_i64, "vmm_cross_attention_bwd_scratch": c_i64, "vmm_linattn_block_workspace": c_i64, "vmm_conv3x3_wgrad_bf16x3_workspace": c_i64, "vmm_conv1x1_wgrad_bf16x3_workspace": c_i64, "vmm_conv_wgrad_tap_workspace": c_i64, "vmm_qkv_bwd_workspace": c_i64, "vmm_temporal_block_bwd_workspace": c_i64, "vmm_linattn_block_bwd_workspace": c_i64, "vmm_groupnorm_bwd_scratch": c_i64}  # everything else returns int (0 = ok)
 
 _lib = None
 

@@ -1,0 +1,187 @@
+"""The global gradient norm over many tensors, clipping by it, and an Adam step on the clipped gradient (csrc/grad_clip.hip).
+
+The reference's loop steps ``torch.optim.Adam`` as it is (vddp.py:1481, 1629-1633); these are what it takes to train a recurrent encoder with it:
+``clip_grad_norm_`` in front of an optimizer of the caller's own, ``ClippedAdam`` -- the same update with the clipping inside, so that it costs no pass
+over the gradients -- or ``DataParallelTrainer(max_grad_norm=...)``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from operator import attrgetter
+from typing import Iterable, List, Optional, Sequence
+
+import torch
+
+from . import _native as N
+
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_dtype = attrgetter("dtype")
+
+
+def on_device(index: int):
+    """The device of a call's tensors made current for its launches, where another one is."""
+    return torch.cuda.device(index if index != torch.cuda.current_device() else -1)
+
+
+def _same_device(tensors: Sequence[torch.Tensor], what: str) -> int:
+    places = set(map(torch.Tensor.get_device, tensors))
+    if len(places) != 1:
+        raise ValueError(f"{what}: the tensors are on several devices")
+    (index,) = places
+    if index < 0 or not tensors[0].is_cuda:
+        raise N.NativeError(f"{what}: tensors must live on the GPU (there is no CPU path)")
+    return index
+
+
+def _check_grads(tensors: Sequence[torch.Tensor], what: str) -> int:
+    bad = set(map(_dtype, tensors)) - set(TYPES)
+    if bad:
+        raise TypeError(f"{what}: float32, bfloat16 or float16 tensors, got {sorted(map(str, bad))}")
+    if not all(map(torch.Tensor.is_contiguous, tensors)):
+        raise ValueError(f"{what}: tensors must be contiguous")
+    return _same_device(tensors, what)
+
+
+def _as_list(tensors, what: str) -> List[torch.Tensor]:
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: expected tensors, got {type(t).__name__}")
+    return tensors
+
+
+def _grad_jobs(tensors: Sequence[torch.Tensor]):
+    jobs = (N.GradJob * len(tensors))()
+    for job, p, n, t in zip(jobs, map(torch.Tensor.data_ptr, tensors), map(torch.Tensor.numel, tensors), map(_dtype, tensors)):
+        job.g, job.n, job.type = p, n, TYPES[t]
+    return jobs
+
+
+def _norm(jobs, n: int, max_norm: float, device: int, scale: float = 1.0) -> torch.Tensor:
+    """(norm, factor) on the device; max_norm <= 0: the factor is one."""
+    lib = N.lib()
+    size = lib.vmm_grad_norm_workspace(jobs, n)
+    if size < 0:
+        raise ValueError("gradient norm: a tensor that is not aligned to its type")
+    work = torch.empty(size // 8 + 1, dtype=torch.float64, device=device)  # (the last one holds the two results)
+    out = work[size // 8:].view(torch.float32)
+    N.check(lib.vmm_grad_norm(jobs, n, scale, max_norm, None, work.data_ptr(), out.data_ptr(), C.c_void_p(torch.cuda.current_stream().cuda_stream)),
+            "vmm_grad_norm")
+    return out
+
+
+@torch.no_grad()
+def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
+    """sqrt of the sum of all squares of `grads` (any mixture of float32, bfloat16, float16), as a float32 scalar on their device; sums are held in 64 bits
+    and have the same bits every time.  No tensors: a zero on the CPU."""
+    grads = _as_list(grads, "grad_norm")
+    if not grads:
+        return torch.zeros(())
+    index = _check_grads(grads, "grad_norm")
+    with on_device(index):
+        return _norm(_grad_jobs(grads), len(grads), 0.0, index)[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(grads: Iterable[torch.Tensor], max_norm: float) -> torch.Tensor:
+    """Scales `grads` (the gradient tensors themselves) in place by min(1, max_norm / (norm + 1e-6)) and returns the norm they had, as a float32 scalar on
+    their device -- torch.nn.utils.clip_grad_norm_ without its host work; nothing is read or written a second time where the norm is within the bound.
+    A NaN norm makes every gradient NaN, an infinite one makes the finite ones zero, as there.  Tensors must not overlap."""
+    grads = _as_list(grads, "clip_grad_norm_")
+    max_norm = float(max_norm)
+    if not max_norm > 0.0:
+        raise ValueError(f"clip_grad_norm_: max_norm must be positive, got {max_norm}")
+    if not grads:
+        return torch.zeros(())
+    index = _check_grads(grads, "clip_grad_norm_")
+    with on_device(index):
+        jobs = _grad_jobs(grads)
+        out = _norm(jobs, len(grads), max_norm, index)
+        code = N.lib().vmm_grad_clip(jobs, len(grads), out.data_ptr(), C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        if code == -2:
+            raise ValueError("clip_grad_norm_: tensors overlap in memory")
+        N.check(code, "vmm_grad_clip")
+        torch.autograd.graph.increment_version(grads)  # written through raw pointers
+    return out[0]
+
+
+class ClippedAdam:
+    """Adam (the update of torch.optim.Adam without weight decay or amsgrad) on gradients clipped by their global norm.
+
+    params: float32 tensors, kept contiguous; exp_avgs / exp_avg_sqs: their moments (zeros where not given), step: the updates they have had.
+    max_norm None: no clipping.  The optimizer keeps one table of its tensors; ``step`` re-reads the addresses, so parameters may be re-homed
+    (``p.data = ...``) but not resized."""
+
+    def __init__(self, params: Iterable[torch.Tensor], lr: float = 1e-4, betas=(0.9, 0.999), eps: float = 1e-8, max_norm: Optional[float] = None, *,
+                 exp_avgs: Optional[Iterable[torch.Tensor]] = None, exp_avg_sqs: Optional[Iterable[torch.Tensor]] = None, step: int = 0):
+        self.params = _as_list(params, "ClippedAdam")
+        if not self.params:
+            raise ValueError("ClippedAdam: no parameters")
+        if max_norm is not None and not max_norm > 0.0:
+            raise ValueError(f"ClippedAdam: max_norm must be positive or None, got {max_norm}")
+        if not (lr >= 0.0 and eps >= 0.0 and all(0.0 <= b < 1.0 for b in betas) and len(betas) == 2 and step >= 0):
+            raise ValueError(f"ClippedAdam: lr {lr}, betas {betas}, eps {eps}, step {step}")
+        self.lr, self.betas, self.eps, self.max_norm, self.steps_taken = lr, tuple(betas), eps, max_norm, int(step)
+        self.exp_avgs = [torch.zeros_like(p, memory_format=torch.contiguous_format) for p in self.params] if exp_avgs is None else _as_list(exp_avgs, "ClippedAdam")
+        self.exp_avg_sqs = [torch.zeros_like(p, memory_format=torch.contiguous_format) for p in self.params] if exp_avg_sqs is None \
+            else _as_list(exp_avg_sqs, "ClippedAdam")
+        self.exp_avgs, self.exp_avg_sqs = [m.detach() for m in self.exp_avgs], [v.detach() for v in self.exp_avg_sqs]
+        self._sizes = list(map(torch.Tensor.numel, self.params))
+        for name, ts in (("params", self.params), ("exp_avgs", self.exp_avgs), ("exp_avg_sqs", self.exp_avg_sqs)):
+            if len(ts) != len(self.params) or list(map(torch.Tensor.numel, ts)) != self._sizes:
+                raise ValueError(f"ClippedAdam: {name} do not fit the parameters")
+        self._device = self._check_own()
+        self._jobs = (N.ClipAdamJob * len(self.params))()
+        for job, m, v, n in zip(self._jobs, self.exp_avgs, self.exp_avg_sqs, self._sizes):
+            job.m, job.v, job.n = m.data_ptr(), v.data_ptr(), n
+        self._at: List[int] = []
+
+    def _check_own(self) -> int:
+        every = self.params + self.exp_avgs + self.exp_avg_sqs
+        if set(map(_dtype, every)) != {torch.float32}:
+            raise TypeError("ClippedAdam: parameters and moments must be float32")
+        if not all(map(torch.Tensor.is_contiguous, every)):
+            raise ValueError("ClippedAdam: parameters and moments must be contiguous")
+        return _same_device(every, "ClippedAdam")
+
+    @torch.no_grad()
+    def step(self, grads: Optional[Iterable[Optional[torch.Tensor]]] = None) -> torch.Tensor:
+        """One update from `grads` (one per parameter; default: every ``p.grad``; None: that parameter stays as it is, and its moments too).
+        Returns the gradients' global norm before clipping, a float32 scalar on the device."""
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError(f"ClippedAdam.step: {len(grads)} gradients for {len(self.params)} parameters")
+        here = [i for i, g in enumerate(grads) if g is not None]
+        if len(here) < len(grads):
+            grads = [grads[i] for i in here]
+            if not grads:
+                return torch.zeros((), device=self._device)
+        sizes = self._sizes if len(here) == len(self._sizes) else [self._sizes[i] for i in here]
+        if list(map(torch.Tensor.numel, grads)) != sizes:
+            raise ValueError("ClippedAdam.step: gradients do not fit the parameters")
+        if _check_grads(grads, "ClippedAdam.step") != self._device:
+            raise ValueError("ClippedAdam.step: gradients and parameters are on different devices")
+        at = list(map(torch.Tensor.data_ptr, self.params))
+        if at != self._at:  # first step, or parameters were re-homed
+            if self._check_own() != self._device or list(map(torch.Tensor.numel, self.params)) != self._sizes:
+                raise ValueError("ClippedAdam.step: parameters were moved to another device or resized")
+            for job, p in zip(self._jobs, at):
+                job.p = p
+            self._at = at
+        with on_device(self._device):
+            jobs = self._jobs
+            if len(here) < len(self.params):
+                jobs = (N.ClipAdamJob * len(here))(*[self._jobs[i] for i in here])
+            norm_jobs = _grad_jobs(grads)
+            for job, g in zip(jobs, norm_jobs):
+                job.g, job.type = g.g, g.type
+            out = _norm(norm_jobs, len(grads), self.max_norm or 0.0, self._device)
+            code = N.lib().vmm_adam_step_clipped(jobs, len(here), self.lr, self.betas[0], self.betas[1], self.eps, self.steps_taken + 1, 1.0, out.data_ptr(),
+                                                 None, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+            if code == -2:
+                raise ValueError("ClippedAdam.step: parameters, moments or gradients overlap in memory")
+            N.check(code, "vmm_adam_step_clipped")
+        self.steps_taken += 1
+        written = self.params if len(here) == len(self.params) else [self.params[i] for i in here]
+        torch.autograd.graph.increment_version(written)  # written through raw pointers
+        return out[0]
