@@ -15,6 +15,7 @@
 #ifndef VMM_KERNELS_H
 #define VMM_KERNELS_H
 #include <stdint.h>
+#include "vmm_sequence.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -767,7 +768,8 @@ int vmm_conv_wgrad_tap_fp16(const vmm_conv_desc* d, const float* dy, int32_t ldd
 int vmm_conv_igemm_fp16(const vmm_conv_desc* d, vmm_stream_t stream);
 int vmm_conv_igemm_fp16_batched(const vmm_conv_desc* descs, int32_t n, vmm_stream_t stream);
 
-/* ==== operators of sequence encoders and of their training.  `type` of a buffer: 0 fp32, 1 bf16, 2 IEEE half; strides count values of that type. ==== */
+/* ==== operators of sequence encoders and of their training (argument structs: vmm_sequence.h).  `type` of a buffer: 0 fp32, 1 bf16, 2 IEEE half;
+ * strides count values of that type. ==== */
 
 /* ---- gated linear recurrence over time, beside vmm_gru_recurrent: no product inside the loop, so the time axis is scanned in parallel.
  *   f = sigmoid(gate),  h_t = f_t h_(t-1) + (1 - f_t) x_t  for t < lengths[b],  y_t = h_t;   y = 0 and the state stands still behind the length.
@@ -778,19 +780,6 @@ int vmm_conv_igemm_fp16_batched(const vmm_conv_desc* descs, int32_t n, vmm_strea
  * dy, dh_last (NULL = zero), dx, dgate, dh0 (each may be NULL) as the tensors they belong to.
  * workspace: vmm_gated_scan_workspace bytes, 16-byte aligned, contents irrelevant, for one call at a time; NULL where that is 0.  The result does
  * not depend on how workgroups fall: the same bits every time. */
-typedef struct vmm_gated_scan_desc {
-  const void* x; int64_t x_batch, x_row;
-  const void* gate; int64_t gate_batch, gate_row;
-  void* y; int64_t y_batch, y_row;
-  const float* h0; float* h_last; const int32_t* lengths; float* states;
-  const void* dy; int64_t dy_batch, dy_row;
-  void* dx; int64_t dx_batch, dx_row;
-  void* dgate; int64_t dgate_batch, dgate_row;
-  const float* dh_last; float* dh0;
-  void* workspace;
-  int64_t L;
-  int32_t B, D, type;
-} vmm_gated_scan_desc;
 int64_t vmm_gated_scan_states(const vmm_gated_scan_desc* d);
 int64_t vmm_gated_scan_workspace(const vmm_gated_scan_desc* d, int32_t backward);
 int vmm_gated_scan(const vmm_gated_scan_desc* d, vmm_stream_t stream);
@@ -803,18 +792,6 @@ int vmm_gated_scan_bwd(const vmm_gated_scan_desc* d, vmm_stream_t stream);
  *   du = dh act(g), dg = dh u act'(g) (rounded to `type`: they are the operands of the products below),
  *   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dbg, dbu = column sums.   dx, (dWg, dWu), (dbg, dbu): each pair may be NULL; they are WRITTEN.
  * workspace: vmm_gated_ff_workspace bytes, 16-byte aligned, contents irrelevant, for one call at a time; NULL where that is 0. */
-typedef struct vmm_gated_ff_desc {
-  const void* x; int64_t ldx;
-  const void* w_gate; const void* w_up; const void* b_gate; const void* b_up;
-  void* h; int64_t ldh;
-  float* g_pre; float* u_pre;
-  const void* dh; int64_t lddh;
-  void* dx; int64_t lddx;
-  void* dw_gate; void* dw_up; void* db_gate; void* db_up;
-  void* workspace;
-  int64_t M;
-  int32_t K, F, type, act;
-} vmm_gated_ff_desc;
 int64_t vmm_gated_ff_workspace(const vmm_gated_ff_desc* d, int32_t backward);
 int vmm_gated_ff(const vmm_gated_ff_desc* d, vmm_stream_t stream);
 int vmm_gated_ff_bwd(const vmm_gated_ff_desc* d, vmm_stream_t stream);
@@ -826,8 +803,6 @@ int vmm_gated_ff_bwd(const vmm_gated_ff_desc* d, vmm_stream_t stream);
  *   vmm_grad_clip          g *= clip[1] in place (clip = out above); nothing is touched where the factor is 1
  *   vmm_adam_step_clipped  vmm_adam_step on grad_scale * clip[1] * g, g of any type; with a scaler's state as vmm_adam_step_scaled (step is not read).
  * Jobs of a writing call must not overlap: -2. */
-typedef struct vmm_grad_job { void* g; int64_t n; int32_t type; int32_t reserved; } vmm_grad_job;
-typedef struct vmm_clip_adam_job { float* p; const void* g; float* m; float* v; int64_t n; int32_t type; int32_t reserved; } vmm_clip_adam_job;
 int64_t vmm_grad_norm_workspace(const vmm_grad_job* jobs, int32_t njobs);
 int vmm_grad_norm(const vmm_grad_job* jobs, int32_t njobs, float scale, float max_norm, float* scaler_state, void* workspace, float* out,
                   vmm_stream_t stream);
