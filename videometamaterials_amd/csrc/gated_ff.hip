@@ -3,90 +3,66 @@
 //   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) u
 //   dg = dh u act'(g),  du = dh act(g),  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dbg = sum_m dg,  dbu = sum_m du
 //
-// Four matrix products of 2 M K F operations in the forward and backward each but for one half: 4 M K F forward, 8 M K F backward.
+// Matrix products bound it: 4 M K F operations forward, 8 M K F backward.  All of them are one kernel, out(i, j) = sum_k A(i, k) B(j, k) over 16-bit
+// operands with fp32 sums, whose operands may be stored with either index contiguous; a product may be the sum of several parts.
+//   forward   A = x, B = rows of Wg and Wu side by side in one tile: a wave holds the same places of g and u, so activation and product need no exchange
+//   dx        A = dg, B = Wg (stored [k][j]), then the part of du and Wu
+//   dW        A = dg (stored [k][i]), B = x (stored [k][j]);  gate and up side by side in the grid
+// fp32 operands are split into three bf16 parts without a remainder (24 = 3 x 8 bits), and a product is the sum of the six parts that reach 2^-16 of it,
+// small ones first; what is left out is below 2^-22.  That is six matrix passes at 16 times the rate of fp32 ones.
+//
+// A tile step is 64 reduced indexes.  It goes from memory to LDS directly (buffer loads with an LDS destination: no registers, and what lies
+// outside the operand arrives as zero), into the one of two buffers that the matrix instructions do not read.  Such a load fills 1 KiB of LDS in lane order,
+// so the banks are spread by which 16 bytes each lane FETCHES: row-contiguous operands swap 16-byte pieces by the row's lower three bits (read back with
+// 16-byte reads), column-contiguous ones by the lower two bits of k (read back with the transposing 8-byte reads).
 #include "vmm_common.h"
 #include "../../include/vmm_kernels.h"
 
 namespace {
+
+typedef unsigned short u16;
+typedef __attribute__((address_space(3))) void lds_void;
 
 template <int TYPE> struct Elem;
 template <> struct Elem<0> { typedef float T; static constexpr int PLANES = 3; };
 template <> struct Elem<1> { typedef __bf16 T; static constexpr int PLANES = 1; };
 template <> struct Elem<2> { typedef _Float16 T; static constexpr int PLANES = 1; };
 
-template <int TYPE>
+template <bool HALF>
 __device__ __forceinline__ f32x16 mfma(const uint4& a, const uint4& b, f32x16 c) {
-  if constexpr (TYPE == 2) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vmm_f16x8, a), __builtin_bit_cast(vmm_f16x8, b), c, 0, 0, 0);
+  if constexpr (HALF) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vmm_f16x8, a), __builtin_bit_cast(vmm_f16x8, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vmm_bf16x8, a), __builtin_bit_cast(vmm_bf16x8, b), c, 0, 0, 0);
 }
 
-// One operand of a product: `rows` x `red` (the reduced index); value (r, k) at p[r ld + k], or p[k ld + r] where COL.
-struct Operand { const void* p; long long ld, rows, red; };
+constexpr int BK = 64;          // reduced indexes of a step
+constexpr int MAX_PARTS = 12;   // dx in fp32: two products of six parts
 
-// A fp32 value as three bf16 parts, x = h + m + l without a remainder: 24 bits of significand are 3 x 8.
-__device__ __forceinline__ void thirds(float x, unsigned short& h, unsigned short& m, unsigned short& l) {
-  const unsigned a = __float_as_uint(x) & 0xffff0000u;
-  const float r = x - __uint_as_float(a);
-  const unsigned b = __float_as_uint(r) & 0xffff0000u;
-  const float s = r - __uint_as_float(b);
-  h = a >> 16; m = b >> 16; l = __float_as_uint(s) >> 16;
+// One product (or two of one shape, dWg and dWu).  A: rows x red, B: cols x red; strides in values, multiples of 8 at 16-byte aligned addresses.
+struct Gemm {
+  const u16* a[MAX_PARTS];
+  const u16* b[MAX_PARTS];
+  const u16* b2[6];                 // forward: the parts of Wu
+  long long lda, ldb, rows, cols, red;
+  int parts, splits;                // the reduced length (of all parts) is cut into `splits` runs
+  long long tiles_m, tiles_n;
+  void* out[2]; long long ldo;      // one run
+  float* partial;                   // several: [product][run][rows][cols], forward [run][2][rows][cols]
+  // forward
+  const void* b_gate; const void* b_up; float* g_pre; float* u_pre; int act;
+};
+
+// a value that is the same in every lane, in a scalar register: integer divisions leave theirs in vector registers, and a buffer descriptor made from
+// such values would be re-read lane by lane
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const u16* uniform(const u16* p) {
+  const unsigned long long v = (unsigned long long)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+  return (const u16*)((unsigned long long)hi << 32 | lo);
 }
 
-constexpr int BM = 128, BK = 32, LDK = BK + 8;  // tile rows, reduced indexes of a step, row pitch in LDS (two-byte values)
-
-// tile[plane][r][k] <- rows r0 .. r0 + ROWS, reduced k0 .. k0 + BK; zero outside
-template <int TYPE, bool COL, int ROWS>
-__device__ __forceinline__ void stage(const Operand& o, long long r0, long long k0, unsigned short* tile) {
-  typedef typename Elem<TYPE>::T T;
-  const T* p = (const T*)o.p;
-  for (int c = threadIdx.x; c < ROWS * BK / 8; c += 256) {
-    const int r = COL ? (c % (ROWS / 8)) * 8 : c / (BK / 8), k = COL ? c / (ROWS / 8) : (c % (BK / 8)) * 8;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int rr = COL ? r + j : r, kk = COL ? k : k + j;
-      const long long gr = r0 + rr, gk = k0 + kk;
-      const bool in = gr < o.rows && gk < o.red;
-      const T v = in ? p[COL ? gk * o.ld + gr : gr * o.ld + gk] : (T)0.f;
-      unsigned short* t = tile + rr * LDK + kk;
-      if constexpr (TYPE == 0) thirds(v, t[0], t[ROWS * LDK], t[2 * ROWS * LDK]);
-      else t[0] = __builtin_bit_cast(unsigned short, v);
-    }
-  }
+__device__ __forceinline__ float act_of(float g, int act) {
+  return act == 0 ? g / (1.0f + expf(-g)) : 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
 }
-
-// acc[mt][nt] += A-tile (rows wm ..) * B-tile (rows wn ..) over BK
-template <int TYPE, int MT, int NT, int AROWS, int BROWS>
-__device__ __forceinline__ void multiply(const unsigned short* ta, const unsigned short* tb, int wm, int wn, f32x16 (&acc)[MT][NT]) {
-  constexpr int P = Elem<TYPE>::PLANES;
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int ks = 0; ks < BK / 16; ++ks) {
-    uint4 a[MT][P], b[NT][P];
-    const int k = ks * 16 + (lane >> 5) * 8;
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i) a[i][p] = *reinterpret_cast<const uint4*>(ta + (p * AROWS + wm + i * 32 + (lane & 31)) * LDK + k);
-#pragma unroll
-      for (int i = 0; i < NT; ++i) b[i][p] = *reinterpret_cast<const uint4*>(tb + (p * BROWS + wn + i * 32 + (lane & 31)) * LDK + k);
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        if constexpr (P == 3) {  // the products of the parts down to 2^-16 of the largest, small ones first; what is left out is below 2^-22
-          acc[i][j] = mfma<TYPE>(a[i][2], b[j][0], acc[i][j]);
-          acc[i][j] = mfma<TYPE>(a[i][0], b[j][2], acc[i][j]);
-          acc[i][j] = mfma<TYPE>(a[i][1], b[j][1], acc[i][j]);
-          acc[i][j] = mfma<TYPE>(a[i][1], b[j][0], acc[i][j]);
-          acc[i][j] = mfma<TYPE>(a[i][0], b[j][1], acc[i][j]);
-        }
-        acc[i][j] = mfma<TYPE>(a[i][0], b[j][0], acc[i][j]);
-      }
-  }
-}
-
-__device__ __forceinline__ float act_of(float g, int act) { return act == 0 ? g / (1.0f + expf(-g)) : 0.5f * g * (1.0f + erff(g * 0.70710678118654752f)); }
 __device__ __forceinline__ void act_both(float g, int act, float& a, float& slope) {
   if (act == 0) {
     const float p = 1.0f / (1.0f + expf(-g));
@@ -102,67 +78,260 @@ __device__ __forceinline__ void act_both(float g, int act, float& a, float& slop
 // row of accumulator register r of a 32 x 32 tile (its column is the lane's lower five bits)
 __device__ __forceinline__ int acc_row(int r) { return (r >> 2) * 8 + ((threadIdx.x & 63) >> 5) * 4 + (r & 3); }
 
-// ---- forward: 128 rows x 64 columns of both projections a workgroup; each of 2 x 2 waves holds the same 64 x 32 of g and u, so that the activation and
-// the product need no exchange
-template <int TYPE>
-__global__ __launch_bounds__(256) void ff_fwd_kernel(const vmm_gated_ff_desc d) {
-  typedef typename Elem<TYPE>::T T;
-  constexpr int P = Elem<TYPE>::PLANES, BF = 64;
-  __shared__ __attribute__((aligned(16))) unsigned short ta[P * BM * LDK], tg[P * BF * LDK], tu[P * BF * LDK];
-  const long long m0 = (long long)blockIdx.x * BM;
-  const int f0 = blockIdx.y * BF;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = (wave & 1) * 64, wf = (wave >> 1) * 32;
-  const Operand x = {d.x, d.ldx, d.M, d.K}, wg = {d.w_gate, d.K, d.F, d.K}, wu = {d.w_up, d.K, d.F, d.K};
-  f32x16 g[2][1] = {}, u[2][1] = {};
-  for (int k0 = 0; k0 < d.K; k0 += BK) {
-    stage<TYPE, false, BM>(x, m0, k0, ta);
-    stage<TYPE, false, BF>(wg, f0, k0, tg);
-    stage<TYPE, false, BF>(wu, f0, k0, tu);
-    __syncthreads();
-    multiply<TYPE, 2, 1, BM, BF>(ta, tg, wm, wf, g);
-    multiply<TYPE, 2, 1, BM, BF>(ta, tu, wm, wf, u);
-    __syncthreads();
-  }
-  const int f = f0 + wf + (lane & 31);
-  if (f >= d.F) return;
-  const float bg = d.b_gate ? (float)((const T*)d.b_gate)[f] : 0.f, bu = d.b_up ? (float)((const T*)d.b_up)[f] : 0.f;
+// ---- one operand's tile of R rows.  Every wave issues R / 8 / WAVES loads of 1 KiB.
+template <bool COL, int R, int WAVES>
+struct Loader {
+  static constexpr int LOADS = R / 8 / WAVES;
+  unsigned off[LOADS];  // byte offset of this lane's 16 bytes from the tile's first value
+  int kc;               // row-contiguous: first k of the lane's piece
+  long long ld, left;
+  // r0: first row of the tile of the `rows`; FOLD: rows 32..63 of every 64 are rows 0..31 of the same 32 in a second matrix
+  template <bool FOLD>
+  __device__ __forceinline__ void init(long long r0, long long rows, long long ld_) {
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    ld = ld_;
+    left = rows - r0;
+    kc = ((lane & 7) ^ (lane >> 3)) * 8;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const long long m = m0 + wm + i * 32 + acc_row(r);
-      if (m >= d.M) continue;
-      const float gv = g[i][0][r] + bg, uv = u[i][0][r] + bu;
-      ((T*)d.h)[m * d.ldh + f] = (T)(act_of(gv, d.act) * uv);
-      if (d.g_pre) {
-        d.g_pre[m * d.F + f] = gv;
-        d.u_pre[m * d.F + f] = uv;
+    for (int i = 0; i < LOADS; ++i) {
+      const int piece = (wave * LOADS + i) * 64 + lane;  // of 16 bytes, in LDS order
+      if constexpr (COL) {
+        const int k = piece / (R / 8), c = (piece % (R / 8)) ^ ((k & 3) << 2);
+        off[i] = c * 8 < left ? (unsigned)(k * ld * 2 + c * 16) : 0xfffffff0u;
+      } else {
+        int r = piece / 8;
+        if constexpr (FOLD) r = (r >> 6) * 32 + (r & 31);
+        off[i] = r < left ? (unsigned)(r * ld * 2 + kc * 2) : 0xfffffff0u;
       }
     }
+  }
+  // p: the tile's first value; k0: reduced index of the step, of `red`
+  __device__ __forceinline__ void load(const u16* p, long long k0, long long red, u16* tile, int i) const {
+    const long long rest = red - k0;
+    const u16* base = p + (COL ? k0 * ld : k0);
+    const unsigned size = COL ? (unsigned)((rest < BK ? rest : BK) * ld * 2) : 0xfffffff0u;  // (rows outside have an offset that no size reaches)
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(base), 0, (int)size, 0x00027000);
+    const int wave = uniform(threadIdx.x >> 6);
+    unsigned o = off[i];
+    if (!COL && kc >= rest) o = 0xfffffff0u;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(tile + (wave * LOADS + i) * 512), 16, o, 0, 0, 0);
+  }
+};
+
+// fragment of 32 rows from r0 on, reduced indexes ks * 16 ..
+template <bool COL, int R>
+__device__ __forceinline__ uint4 fragment(const u16* tile, int r0, int ks) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (COL) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    const int i = lane & 15, k = ks * 16 + (lane >> 5) * 8 + (i >> 2), r = r0 + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
+    const u16* at = tile + k * R + (((r >> 3) ^ ((i >> 2) << 2)) << 3) + (r & 7);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 4 * R));
+    const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
+    return make_uint4(l.x, l.y, h.x, h.y);
+  } else {
+    const int r = r0 + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ (r & 7);
+    return *reinterpret_cast<const uint4*>(tile + r * BK + c * 8);
+  }
 }
 
-// ---- backward, first: dg and du (rounded to the type, as operands) and the partial column sums of a run of rows
-constexpr int ROW_RUN = 64;
+// ---- out = A B^T.  BIG: 256 x 256 tiles, 8 waves of 128 x 64; else 128 x 128 tiles, 4 waves of 64 x 64.
+template <int TYPE, bool ACOL, bool BCOL, bool GATED, bool BIG>
+__global__ __launch_bounds__(BIG ? 512 : 256, BIG ? 2 : 2) void ff_gemm_kernel(const Gemm q) {
+  typedef typename Elem<TYPE>::T T;
+  constexpr bool HALF = TYPE == 2;
+  constexpr int R = BIG ? 256 : 128, WAVES = BIG ? 8 : 4, WM = BIG ? 128 : 64, MT = WM / 32;
+  __shared__ __attribute__((aligned(16))) u16 a0[R * BK], b0[R * BK], a1[R * BK], b1[R * BK];
+  // Consecutive workgroups go to different XCDs: each XCD gets a run of tiles that are neighbours, 8 rows of tiles at a time, and finds its operands
+  // in its own L2.
+  const unsigned tiles = (unsigned)(q.tiles_m * q.tiles_n), per = (tiles + 7) / 8, t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (t >= tiles) return;
+  const unsigned in_all = 8 * (unsigned)q.tiles_n, band = t / in_all, bm = min(8u, (unsigned)q.tiles_m - band * 8), in_band = t - band * in_all;
+  const long long m0 = (long long)uniform(band * 8 + in_band % bm) * R, n0 = (long long)uniform(in_band / bm) * (GATED ? R / 2 : R);
+  const int run = uniform(blockIdx.y % q.splits), prod = uniform(blockIdx.y / q.splits);
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = BIG ? (wave & 1) * 128 : (wave & 1) * 64, wn = (wave >> 1) * 64;
+
+  Loader<ACOL, R, WAVES> la;
+  Loader<BCOL, R, WAVES> lb;
+  la.template init<false>(m0, q.rows, q.lda);
+  lb.template init<GATED>(n0, q.cols, q.ldb);
+  const int steps = (int)((q.red + BK - 1) / BK), units = steps * q.parts;
+  const int u0 = uniform((int)((long long)units * run / q.splits)), u1 = uniform((int)((long long)units * (run + 1) / q.splits));
+  int part = uniform(u0 / max(steps, 1)), step = u0 - part * steps;
+  const long long ao = ACOL ? m0 : m0 * q.lda, bo = BCOL ? n0 : n0 * q.ldb;
+  auto fetch = [&](u16* ta, u16* tb) {
+    const u16* pa = q.a[prod * q.parts + part] + ao;
+    const u16* pb = q.b[prod * q.parts + part] + bo;
+    const long long k0 = (long long)step * BK;
+#pragma unroll
+    for (int i = 0; i < la.LOADS; ++i) la.load(pa, k0, q.red, ta, i);
+#pragma unroll
+    for (int i = 0; i < lb.LOADS; ++i) {
+      const u16* p = pb;
+      if constexpr (GATED) {
+        const int row = (wave * lb.LOADS + i) * 8;  // of the tile: eight rows a load
+        if (row & 32) p = q.b2[part] + bo;
+      }
+      lb.load(p, k0, q.red, tb, i);
+    }
+    if (++step == steps) { step = 0; ++part; }
+  };
+  f32x16 acc[MT][2] = {};
+  auto compute = [&](const u16* ta, const u16* tb) {
+#pragma unroll
+    for (int ks = 0; ks < BK / 16; ++ks) {
+      uint4 a[MT], b[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) b[j] = fragment<BCOL, R>(tb, wn + j * 32, ks);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) a[i] = fragment<ACOL, R>(ta, wm + i * 32, ks);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma<HALF>(a[i], b[j], acc[i][j]);
+    }
+  };
+  if (u0 < u1) fetch(a0, b0);
+  for (int u = u0; u < u1; u += 2) {
+    __syncthreads();  // this wave's loads have landed, and every wave's after the barrier; nobody reads the other buffer any more
+    if (u + 1 < u1) fetch(a1, b1);
+    compute(a0, b0);
+    if (u + 1 >= u1) break;
+    __syncthreads();
+    if (u + 2 < u1) fetch(a0, b0);
+    compute(a1, b1);
+  }
+
+  if constexpr (GATED) {
+    const long long f = n0 + wn / 2 + (lane & 31);
+    if (f >= q.cols) return;
+    if (q.splits > 1) {
+      float* pg = q.partial + (long long)run * 2 * q.rows * q.cols;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const long long m = m0 + wm + i * 32 + acc_row(r);
+          if (m < q.rows) {
+            pg[m * q.cols + f] = acc[i][0][r];
+            pg[(q.rows + m) * q.cols + f] = acc[i][1][r];
+          }
+        }
+      return;
+    }
+    const float bg = q.b_gate ? (float)((const T*)q.b_gate)[f] : 0.f, bu = q.b_up ? (float)((const T*)q.b_up)[f] : 0.f;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const long long m = m0 + wm + i * 32 + acc_row(r);
+        if (m >= q.rows) continue;
+        const float g = acc[i][0][r] + bg, v = acc[i][1][r] + bu;
+        ((T*)q.out[0])[m * q.ldo + f] = (T)(act_of(g, q.act) * v);
+        if (q.g_pre) {
+          q.g_pre[m * q.cols + f] = g;
+          q.u_pre[m * q.cols + f] = v;
+        }
+      }
+  } else {
+    float* part_out = q.partial + (long long)blockIdx.y * q.rows * q.cols;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const long long m = m0 + wm + i * 32 + acc_row(r), n = n0 + wn + j * 32 + (lane & 31);
+          if (m >= q.rows || n >= q.cols) continue;
+          if (q.splits > 1) part_out[m * q.cols + n] = acc[i][j][r];
+          else ((T*)q.out[prod])[m * q.ldo + n] = (T)acc[i][j][r];
+        }
+  }
+}
+
+// ---- the runs of a split product, added in order
 template <int TYPE>
-__global__ __launch_bounds__(256) void ff_dact_kernel(const vmm_gated_ff_desc d, void* dg_, void* du_, float* __restrict__ sums) {
+__global__ __launch_bounds__(256) void ff_join_kernel(const Gemm q) {
+  typedef typename Elem<TYPE>::T T;
+  const long long n = q.rows * q.cols, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const float* p = q.partial + (long long)blockIdx.y * q.splits * n + i;
+  float s = 0.f;
+  for (int r = 0; r < q.splits; ++r) s += p[r * n];
+  ((T*)q.out[blockIdx.y])[i / q.cols * q.ldo + i % q.cols] = (T)s;
+}
+template <int TYPE>
+__global__ __launch_bounds__(256) void ff_join_gated_kernel(const Gemm q) {
+  typedef typename Elem<TYPE>::T T;
+  const long long n = q.rows * q.cols, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const long long m = i / q.cols, f = i % q.cols;
+  float g = 0.f, u = 0.f;
+  for (int r = 0; r < q.splits; ++r) {
+    g += q.partial[2 * r * n + i];
+    u += q.partial[(2 * r + 1) * n + i];
+  }
+  g += q.b_gate ? (float)((const T*)q.b_gate)[f] : 0.f;
+  u += q.b_up ? (float)((const T*)q.b_up)[f] : 0.f;
+  ((T*)q.out[0])[m * q.ldo + f] = (T)(act_of(g, q.act) * u);
+  if (q.g_pre) { q.g_pre[i] = g; q.u_pre[i] = u; }
+}
+
+// ---- operands: three bf16 parts of fp32 values, or 16-bit values whose rows are not made of whole 16-byte pieces, laid out with padded rows
+struct Layin { const void* src[3]; u16* dst[3]; long long rows[3], ld[3]; int cols, pitch; };
+
+__device__ __forceinline__ void thirds(float x, u16& h, u16& m, u16& l) {
+  const unsigned a = __float_as_uint(x) & 0xffff0000u;
+  const float r = x - __uint_as_float(a);
+  const unsigned b = __float_as_uint(r) & 0xffff0000u;
+  const float s = r - __uint_as_float(b);
+  h = a >> 16; m = b >> 16; l = __float_as_uint(s) >> 16;
+}
+template <int TYPE>
+__device__ __forceinline__ void put(u16* p, long long plane, float v) {
+  if constexpr (TYPE == 0) thirds(v, p[0], p[plane], p[2 * plane]);
+  else *p = __builtin_bit_cast(u16, (typename Elem<TYPE>::T)v);
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void ff_layin_kernel(const Layin a) {
+  typedef typename Elem<TYPE>::T T;
+  const int z = blockIdx.y;
+  const long long n = a.rows[z] * a.pitch;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long r = i / a.pitch;
+    const int c = (int)(i - r * a.pitch);
+    const T v = c < a.cols ? ((const T*)a.src[z])[r * a.ld[z] + c] : (T)0.f;
+    put<TYPE>(a.dst[z] + i, n, (float)v);
+  }
+}
+
+// ---- backward, first: dg and du as operands (rounded to the type, or split) and the partial column sums of a run of rows
+template <int TYPE>
+__global__ __launch_bounds__(256) void ff_dact_kernel(const vmm_gated_ff_desc d, u16* dg, u16* du, int pitch, int run, float* __restrict__ sums) {
   typedef typename Elem<TYPE>::T T;
   const int f = blockIdx.x * 256 + threadIdx.x;
-  if (f >= d.F) return;
-  T* dg = (T*)dg_;
-  T* du = (T*)du_;
+  if (f >= pitch) return;
+  const long long plane = d.M * pitch;
   float sg = 0.f, su = 0.f;
-  const long long m1 = min((long long)d.M, (long long)(blockIdx.y + 1) * ROW_RUN);
-  for (long long m = (long long)blockIdx.y * ROW_RUN; m < m1; ++m) {
-    const float dh = (float)((const T*)d.dh)[m * d.lddh + f];
-    float a, slope;
-    act_both(d.g_pre[m * d.F + f], d.act, a, slope);
-    const float vg = dh * d.u_pre[m * d.F + f] * slope, vu = dh * a;
-    dg[m * d.F + f] = (T)vg;
-    du[m * d.F + f] = (T)vu;
+  const long long m1 = min((long long)d.M, (long long)(blockIdx.y + 1) * run);
+  for (long long m = (long long)blockIdx.y * run; m < m1; ++m) {
+    float vg = 0.f, vu = 0.f;
+    if (f < d.F) {
+      const float dh = (float)((const T*)d.dh)[m * d.lddh + f];
+      float a, slope;
+      act_both(d.g_pre[m * d.F + f], d.act, a, slope);
+      vg = dh * d.u_pre[m * d.F + f] * slope;
+      vu = dh * a;
+    }
+    put<TYPE>(dg + m * pitch + f, plane, vg);
+    put<TYPE>(du + m * pitch + f, plane, vu);
     sg += vg;
     su += vu;
   }
-  if (sums) {
+  if (sums && f < d.F) {
     sums[(long long)blockIdx.y * 2 * d.F + f] = sg;
     sums[(long long)blockIdx.y * 2 * d.F + d.F + f] = su;
   }
@@ -178,87 +347,177 @@ __global__ __launch_bounds__(256) void ff_dbias_kernel(const vmm_gated_ff_desc d
   else if (d.db_up) ((T*)d.db_up)[f - d.F] = (T)s;
 }
 
-// ---- backward products: out[i][j] = sum over the parts and k of A(i, k) B(j, k)
-struct Product { Operand a[2], b[2]; int parts; void* out[2]; long long ldo; };
-template <int TYPE, bool ACOL>
-__global__ __launch_bounds__(256) void ff_product_kernel(const Product p) {
-  typedef typename Elem<TYPE>::T T;
-  constexpr int P = Elem<TYPE>::PLANES;
-  __shared__ __attribute__((aligned(16))) unsigned short ta[P * BM * LDK], tb[P * BM * LDK];
-  const long long m0 = (long long)blockIdx.x * BM, n0 = (long long)blockIdx.y * BM;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-  f32x16 acc[2][2] = {};
-  const int z = blockIdx.z;  // with one part, z picks the product
-  for (int part = 0; part < p.parts; ++part) {
-    const Operand a = p.a[z + part], b = p.b[z + part];
-    for (long long k0 = 0; k0 < a.red; k0 += BK) {
-      stage<TYPE, ACOL, BM>(a, m0, k0, ta);
-      stage<TYPE, true, BM>(b, n0, k0, tb);
-      __syncthreads();
-      multiply<TYPE, 2, 2, BM, BM>(ta, tb, wm, wn, acc);
-      __syncthreads();
-    }
-  }
-  const long long M = p.a[z].rows, N = p.b[z].rows;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const long long m = m0 + wm + i * 32 + acc_row(r), n = n0 + wn + j * 32 + (lane & 31);
-        if (m < M && n < N) ((T*)p.out[z])[m * p.ldo + n] = (T)acc[i][j][r];
-      }
-}
+// ---- host side
 
 inline int esize(int type) { return type == 0 ? 4 : 2; }
-inline long long up16(long long n) { return (n + 15) / 16 * 16; }
+inline long long up(long long n, long long to) { return (n + to - 1) / to * to; }
 
 bool bad_ff(const vmm_gated_ff_desc* d) {
-  return !d || d->M < 0 || d->K < 1 || d->F < 1 || d->M >= (1LL << 31) || d->type < 0 || d->type > 2 || d->act < 0 || d->act > 1;
+  // (K, F < 2^22: a tile of 256 rows is addressed with 32-bit byte offsets)
+  return !d || d->M < 0 || d->K < 1 || d->F < 1 || d->K >= (1 << 22) || d->F >= (1 << 22) || d->M >= (1LL << 31) || d->type < 0 || d->type > 2 ||
+         d->act < 0 || d->act > 1 || d->ldx < 0 || d->ldx >= (1 << 22);
 }
-struct Layout { long long dg, du, sums, bytes; int runs; };
-Layout layout(const vmm_gated_ff_desc* d) {
+
+// The tiles and runs of a product.  Big tiles read LDS 0.75 times per matrix instruction slot where small ones read it as often as it can be read; they
+// are taken where they fill the card.  A product with fewer tiles than CUs is cut along its reduced length, by four steps a run at the least.
+struct Shape { bool big; int splits; };
+Shape shape_of(long long rows, long long cols, bool gated, long long units, int products) {
+  const auto tiles = [&](long long r) { return ((rows + r - 1) / r) * ((cols * (gated ? 2 : 1) + r - 1) / r) * products; };
+  Shape s;
+  s.big = tiles(256) >= 192;
+  const long long t = tiles(s.big ? 256 : 128);
+  long long n = 1;
+  if (t < 256) n = 512 / t;
+  if (n > units / 4) n = units / 4;
+  if (n > 64) n = 64;
+  s.splits = (int)(n < 1 ? 1 : n);
+  return s;
+}
+inline long long units_of(long long red, int parts) { return (red + BK - 1) / BK * parts; }
+
+struct Layout {
+  bool lay;                 // operands are laid out in the workspace
+  int planes, kp, fp, runs, run;
+  long long x, wg, wu, dg, du, sums, partial, bytes;
+  Shape fwd, dx, dw;
+};
+// x as an operand where it is: whole 16-byte pieces
+bool whole(const void* p, long long ld, int cols, int type) { return type != 0 && ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld >= cols; }
+
+Layout layout(const vmm_gated_ff_desc* d, bool backward) {
   Layout l;
-  l.runs = (int)((d->M + ROW_RUN - 1) / ROW_RUN);
-  l.dg = 0;
-  l.du = up16(d->M * d->F * esize(d->type));
-  l.sums = 2 * l.du;
-  l.bytes = l.sums + up16(8LL * l.runs * d->F);
+  l.planes = d->type == 0 ? 3 : 1;
+  const int parts = d->type == 0 ? 6 : 1;
+  l.kp = (int)up(d->K, 8);
+  l.fp = (int)up(d->F, 8);
+  l.lay = !(d->K % 8 == 0 && whole(d->x, d->ldx, d->K, d->type) && whole(d->w_gate, d->K, d->K, d->type) && whole(d->w_up, d->K, d->K, d->type));
+  long long at = 0;
+  const auto take = [&](long long bytes) { const long long o = at; at += up(bytes, 256); return o; };
+  l.x = l.lay ? take(2LL * l.planes * d->M * l.kp) : 0;
+  l.wg = l.lay ? take(2LL * l.planes * d->F * l.kp) : 0;
+  l.wu = l.lay ? take(2LL * l.planes * d->F * l.kp) : 0;
+  l.fwd = shape_of(d->M, d->F, true, units_of(d->K, parts), 1);
+  l.dx = shape_of(d->M, d->K, false, units_of(d->F, 2 * parts), 1);
+  l.dw = shape_of(d->F, d->K, false, units_of(d->M, parts), 2);
+  if (backward) {
+    l.dg = take(2LL * l.planes * d->M * l.fp);
+    l.du = take(2LL * l.planes * d->M * l.fp);
+    l.run = (int)(d->M <= 64 * 1024 ? 64 : up((d->M + 1023) / 1024, 64));
+    l.runs = (int)((d->M + l.run - 1) / l.run);
+    l.sums = take(8LL * l.runs * d->F);
+    const long long px = l.dx.splits > 1 && d->dx ? 4LL * l.dx.splits * d->M * d->K : 0, pw = l.dw.splits > 1 && d->dw_gate ? 8LL * l.dw.splits * d->F * d->K : 0;
+    l.partial = take(px > pw ? px : pw);
+  } else {
+    l.partial = take(l.fwd.splits > 1 ? 8LL * l.fwd.splits * d->M * d->F : 0);
+  }
+  l.bytes = at;
   return l;
 }
 
+template <int TYPE, bool ACOL, bool BCOL, bool GATED>
+int product(Gemm& q, const Shape& sh, int products, hipStream_t s) {
+  const int r = sh.big ? 256 : 128;
+  q.splits = sh.splits;
+  q.tiles_m = (q.rows + r - 1) / r;
+  q.tiles_n = (q.cols * (GATED ? 2 : 1) + r - 1) / r;
+  const long long blocks = (q.tiles_m * q.tiles_n + 7) / 8 * 8;
+  if (blocks >= (1LL << 30) || (q.red + BK - 1) / BK * q.parts >= (1LL << 30)) return -1;
+  const dim3 grid((unsigned)blocks, products * q.splits);
+  if (sh.big) hipLaunchKernelGGL((ff_gemm_kernel<TYPE, ACOL, BCOL, GATED, true>), grid, dim3(512), 0, s, q);
+  else hipLaunchKernelGGL((ff_gemm_kernel<TYPE, ACOL, BCOL, GATED, false>), grid, dim3(256), 0, s, q);
+  VMM_LAUNCH_CHECK();
+  if (q.splits > 1) {
+    const long long n = (q.rows * q.cols + 255) / 256;
+    if (n >= (1LL << 31)) return -1;
+    if constexpr (GATED) hipLaunchKernelGGL(ff_join_gated_kernel<TYPE>, dim3((unsigned)n), dim3(256), 0, s, q);
+    else hipLaunchKernelGGL(ff_join_kernel<TYPE>, dim3((unsigned)n, products), dim3(256), 0, s, q);
+    VMM_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+// which parts of A and B a product is made of, small ones first
+constexpr int PART_A[6] = {2, 0, 1, 1, 0, 0}, PART_B[6] = {0, 2, 1, 0, 1, 0};
+template <int TYPE> int parts_of(int i, bool of_a) { return TYPE == 0 ? (of_a ? PART_A[i] : PART_B[i]) : 0; }
+
+struct Operands { const u16 *x, *wg, *wu; long long ldx, ldw, xplane, wplane; };
 template <int TYPE>
-int forward(const vmm_gated_ff_desc* d, hipStream_t s) {
-  hipLaunchKernelGGL(ff_fwd_kernel<TYPE>, dim3(cdiv(d->M, BM), cdiv(d->F, 64)), dim3(256), 0, s, *d);
+int operands(const vmm_gated_ff_desc* d, const Layout& l, Operands& o, hipStream_t s) {
+  char* w = (char*)d->workspace;
+  if (!l.lay) {
+    o = {(const u16*)d->x, (const u16*)d->w_gate, (const u16*)d->w_up, d->ldx, d->K, 0, 0};
+    return 0;
+  }
+  o = {(const u16*)(w + l.x), (const u16*)(w + l.wg), (const u16*)(w + l.wu), l.kp, l.kp, d->M * l.kp, (long long)d->F * l.kp};
+  const Layin a = {{d->x, d->w_gate, d->w_up}, {(u16*)(w + l.x), (u16*)(w + l.wg), (u16*)(w + l.wu)}, {d->M, d->F, d->F}, {d->ldx, d->K, d->K}, d->K, l.kp};
+  const long long most = (d->M > d->F ? d->M : d->F) * (long long)l.kp;
+  hipLaunchKernelGGL(ff_layin_kernel<TYPE>, dim3((unsigned)min(cdiv(most, 256), 4096), 3), dim3(256), 0, s, a);
   VMM_LAUNCH_CHECK();
   return 0;
 }
 
 template <int TYPE>
+int forward(const vmm_gated_ff_desc* d, hipStream_t s) {
+  constexpr int NP = TYPE == 0 ? 6 : 1;
+  const Layout l = layout(d, false);
+  Operands o;
+  if (const int e = operands<TYPE>(d, l, o, s)) return e;
+  Gemm q = {};
+  for (int i = 0; i < NP; ++i) {
+    q.a[i] = o.x + parts_of<TYPE>(i, true) * o.xplane;
+    q.b[i] = o.wg + parts_of<TYPE>(i, false) * o.wplane;
+    q.b2[i] = o.wu + parts_of<TYPE>(i, false) * o.wplane;
+  }
+  q.lda = o.ldx; q.ldb = o.ldw; q.rows = d->M; q.cols = d->F; q.red = d->K; q.parts = NP;
+  q.out[0] = d->h; q.ldo = d->ldh;
+  q.partial = (float*)((char*)d->workspace + l.partial);
+  q.b_gate = d->b_gate; q.b_up = d->b_up; q.g_pre = d->g_pre; q.u_pre = d->u_pre; q.act = d->act;
+  return product<TYPE, false, false, true>(q, l.fwd, 1, s);
+}
+
+template <int TYPE>
 int backward(const vmm_gated_ff_desc* d, hipStream_t s) {
-  const Layout l = layout(d);
+  constexpr int NP = TYPE == 0 ? 6 : 1;
+  const Layout l = layout(d, true);
   char* w = (char*)d->workspace;
   const bool bias = d->db_gate || d->db_up;
   float* sums = bias ? (float*)(w + l.sums) : nullptr;
+  u16 *dg = (u16*)(w + l.dg), *du = (u16*)(w + l.du);
   if (d->M > 0) {
-    hipLaunchKernelGGL(ff_dact_kernel<TYPE>, dim3(cdiv(d->F, 256), l.runs), dim3(256), 0, s, *d, (void*)(w + l.dg), (void*)(w + l.du), sums);
+    hipLaunchKernelGGL(ff_dact_kernel<TYPE>, dim3(cdiv(l.fp, 256), l.runs), dim3(256), 0, s, *d, dg, du, l.fp, l.run, sums);
     VMM_LAUNCH_CHECK();
   }
   if (bias) {
     hipLaunchKernelGGL(ff_dbias_kernel<TYPE>, dim3(cdiv(2LL * d->F, 256)), dim3(256), 0, s, *d, (const float*)sums, l.runs);
     VMM_LAUNCH_CHECK();
   }
+  Operands o;
+  if (const int e = operands<TYPE>(d, l, o, s)) return e;
+  const long long plane = d->M * l.fp;
   if (d->dx && d->M > 0) {
-    const Product p = {{{w + l.dg, d->F, d->M, d->F}, {w + l.du, d->F, d->M, d->F}}, {{d->w_gate, d->K, d->K, d->F}, {d->w_up, d->K, d->K, d->F}}, 2, {d->dx, nullptr}, d->lddx};
-    hipLaunchKernelGGL((ff_product_kernel<TYPE, false>), dim3(cdiv(d->M, BM), cdiv(d->K, BM), 1), dim3(256), 0, s, p);
-    VMM_LAUNCH_CHECK();
+    Gemm q = {};
+    for (int i = 0; i < NP; ++i) {
+      q.a[2 * i] = dg + parts_of<TYPE>(i, true) * plane;
+      q.b[2 * i] = o.wg + parts_of<TYPE>(i, false) * o.wplane;
+      q.a[2 * i + 1] = du + parts_of<TYPE>(i, true) * plane;
+      q.b[2 * i + 1] = o.wu + parts_of<TYPE>(i, false) * o.wplane;
+    }
+    q.lda = l.fp; q.ldb = o.ldw; q.rows = d->M; q.cols = d->K; q.red = d->F; q.parts = 2 * NP;
+    q.out[0] = d->dx; q.ldo = d->lddx;
+    q.partial = (float*)(w + l.partial);
+    if (const int e = product<TYPE, false, true, false>(q, l.dx, 1, s)) return e;
   }
   if (d->dw_gate) {
-    const Operand x = {d->x, d->ldx, d->K, d->M};
-    const Product p = {{{w + l.dg, d->F, d->F, d->M}, {w + l.du, d->F, d->F, d->M}}, {x, x}, 1, {d->dw_gate, d->dw_up}, d->K};
-    hipLaunchKernelGGL((ff_product_kernel<TYPE, true>), dim3(cdiv(d->F, BM), cdiv(d->K, BM), 2), dim3(256), 0, s, p);
-    VMM_LAUNCH_CHECK();
+    Gemm q = {};
+    for (int i = 0; i < NP; ++i) {
+      q.a[i] = dg + parts_of<TYPE>(i, true) * plane;
+      q.a[NP + i] = du + parts_of<TYPE>(i, true) * plane;
+      q.b[i] = q.b[NP + i] = o.x + parts_of<TYPE>(i, false) * o.xplane;
+    }
+    q.lda = l.fp; q.ldb = o.ldx; q.rows = d->F; q.cols = d->K; q.red = d->M; q.parts = NP;
+    q.out[0] = d->dw_gate; q.out[1] = d->dw_up; q.ldo = d->K;
+    q.partial = (float*)(w + l.partial);
+    if (const int e = product<TYPE, true, true, false>(q, l.dw, 2, s)) return e;
   }
   return 0;
 }
@@ -267,13 +526,14 @@ int backward(const vmm_gated_ff_desc* d, hipStream_t s) {
 
 extern "C" int64_t vmm_gated_ff_workspace(const vmm_gated_ff_desc* d, int32_t backward) {
   if (bad_ff(d)) return -1;
-  return backward ? layout(d).bytes : 0;
+  return layout(d, backward != 0).bytes;
 }
 
 extern "C" int vmm_gated_ff(const vmm_gated_ff_desc* d, vmm_stream_t stream) {
   if (bad_ff(d)) return -1;
   if (d->M == 0) return 0;
   if (!d->x || !d->w_gate || !d->w_up || !d->h || !d->g_pre != !d->u_pre) return -1;
+  if (layout(d, false).bytes > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15))) return -1;
   hipStream_t s = (hipStream_t)stream;
   return d->type == 0 ? forward<0>(d, s) : d->type == 1 ? forward<1>(d, s) : forward<2>(d, s);
 }
@@ -282,7 +542,7 @@ extern "C" int vmm_gated_ff_bwd(const vmm_gated_ff_desc* d, vmm_stream_t stream)
   if (bad_ff(d)) return -1;
   if (!d->dw_gate != !d->dw_up) return -1;
   if (d->M > 0 && (!d->x || !d->w_gate || !d->w_up || !d->dh || !d->g_pre || !d->u_pre)) return -1;
-  if (vmm_gated_ff_workspace(d, 1) > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15))) return -1;
+  if (layout(d, true).bytes > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15))) return -1;
   hipStream_t s = (hipStream_t)stream;
   return d->type == 0 ? backward<0>(d, s) : d->type == 1 ? backward<1>(d, s) : backward<2>(d, s);
 }
