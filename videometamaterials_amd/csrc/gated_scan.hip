@@ -3,29 +3,28 @@
 //   f_t = sigmoid(g_t),   h_t = f_t h_(t-1) + (1 - f_t) x_t,   y_t = h_t
 //   dh_t = dy_t + f_(t+1) dh_(t+1),   dx_t = dh_t (1 - f_t),   dg_t = dh_t (h_(t-1) - x_t) f_t (1 - f_t),   dh0 = f_1 dh_1
 //
-// A step is the map h -> P h + Q with (P, Q) = (f, (1 - f) x), and maps compose: (P2, Q2) o (P1, Q1) = (P2 P1, P2 Q1 + Q2).  So time is cut into pieces
-// whose maps are formed side by side and then joined in order; the backward runs the same machine from the right with c_t = f_t (dy_t + c_(t+1)).
+// A step is the map h -> P h + Q with (P, Q) = (f, (1 - f) x), and maps compose: (P2, Q2) o (P1, Q1) = (P2 P1, P2 Q1 + Q2).  So time is cut into units of
+// 64 steps.  The backward runs the same machine from the end of time with c_t = f_t (dy_t + c_(t+1)), whose maps are (f, f dy).
+//   1. maps     every unit's map, and that of every 16 units (a group)                       reads x and gate (backward: gate and dy)
+//   2. states   the state in front of every unit: maps of the groups before, then of the units before inside the group
+//   3. apply    every unit by itself from that state                                         reads x and gate, writes y
+// A sequence of one unit needs the last alone.  Where there are more than 256 groups, the state in front of every 256th (an anchor) is formed first, so
+// that step 2 goes through 255 groups at the most.  Which maps are joined in which order depends on the sizes alone: the same bits every time.
 //
-// What bounds it: memory.  Forward reads x and gate once and writes y (3 values a step), backward reads x, gate, dy and writes dx, dgate (5).  Nothing
-// is read twice: a tile stays in registers while its carry arrives.
-//   thread   4 adjacent channels x TS steps; f and (1 - f) x in registers
-//   wave     16 channel groups x 4 segments of time; joined with lane exchanges
-//   block    4 waves = 16 segments: a tile of 64 channels x 16 TS steps; wave totals joined through LDS
-//   grid     tiles along time pass the state on through memory: a tile first publishes its own map, then takes the state at the start of its group of
-//            GROUP tiles and the maps published since, and joins them in order.  The last tile of a group publishes the state behind it.  The order in
-//            which maps are joined is fixed by their places, not by who came first, so the result has the same bits every time.
-// A tile waits for earlier tiles only.  Tiles are handed out by a counter in that order, so whoever holds the earliest unfinished one is working on it
-// with all it needs published: every wait ends, however workgroups are placed.  A published value is one 64-bit (map) or 32-bit (state) word that is
-// written whole and is not EMPTY, so it needs no flag and no fence.
+// What bounds it: memory, 3 values a step forward and 5 backward, plus 2 for the maps, which the third step finds in the 256 MB of last-level cache for
+// the most part: it walks time from the end, where step 1 has read last.  Passing states from workgroup to workgroup inside one launch would read all of
+// it once, and was built first; workgroups then poll each other's results past the caches, and 65536 steps of 1024 channels took 192 us (228 us
+// with groups and tiles of 128 steps; 370 us with tiles of 64) where these three launches take 0.17 ms.
 #include "vmm_common.h"
 #include "../../include/vmm_kernels.h"
 
 namespace {
 
-constexpr unsigned EMPTY = 0xffffffffu;  // what the workspace is filled with: a NaN that publish() never writes
 constexpr int V = 4;                     // channels of a thread
 constexpr int CG = 16;                   // channel groups of a tile: rows of 128 bytes in 16 bits, 256 in fp32
-constexpr int STATE_STEP = 64;           // steps between the states that the forward keeps: the backward's tile
+constexpr int UNIT = 64;                 // steps of a unit of time
+constexpr int GROUP = 16;                // units of a group
+constexpr int ANCHOR = 256;              // groups between anchors
 
 template <int TYPE> struct Elem;
 template <> struct Elem<0> { typedef float T; typedef uint4 W; static constexpr unsigned PAD = 0x42D00000u; };
@@ -65,21 +64,21 @@ __device__ __forceinline__ typename Elem<TYPE>::W fill_word(unsigned w) {
   else return make_uint2(w, w);
 }
 
-// Where a thread's V channels are: side by side where accesses of four values are possible (WIDE), else 16 apart, so that the 16 lanes of a row still
-// read 16 neighbours.
+// A thread's V channels inside a tile: side by side where accesses of four values are possible (WIDE), else 16 apart, so that the 16 lanes of a row
+// still read 16 neighbours.  Rows are addressed as a place that is the same for all lanes plus a 32-bit lane offset.
 template <int TYPE, bool WIDE>
 struct Place {
   typedef typename Elem<TYPE>::T T;
   typedef typename Elem<TYPE>::W W;
-  int d0, D;
-  __device__ __forceinline__ Place(int tile, int cg, int D_) : d0(tile * CG * V + (WIDE ? cg * V : cg)), D(D_) {}
+  int d0, D;  // D: channels from the tile's first one on
+  __device__ __forceinline__ Place(int cg, int D_) : d0(WIDE ? cg * V : cg), D(D_) {}
   __device__ __forceinline__ int channel(int j) const { return WIDE ? d0 + j : d0 + j * CG; }
   __device__ __forceinline__ bool has(int j) const { return WIDE ? d0 < D : d0 + j * CG < D; }
-  // row: the address of channel 0 of a step
-  __device__ __forceinline__ W load(const T* row, unsigned pad) const {
+  // row: the address of the tile's first channel, off: of the lane's own beyond it, in bytes
+  __device__ __forceinline__ W load(const char* row, unsigned off, unsigned pad) const {
     if constexpr (WIDE) {
       W r = fill_word<TYPE>(pad);
-      if (d0 < D) r = *reinterpret_cast<const W*>(row + d0);
+      if (d0 < D) r = *reinterpret_cast<const W*>(row + off);
       return r;
     } else {
       unsigned w[V];
@@ -87,24 +86,25 @@ struct Place {
       for (int j = 0; j < V; ++j) {
         w[j] = pad;
         if (has(j)) {
-          if constexpr (TYPE == 0) w[j] = __builtin_bit_cast(unsigned, row[channel(j)]);
-          else w[j] = __builtin_bit_cast(unsigned short, row[channel(j)]);
+          const T* p = reinterpret_cast<const T*>(row + off) + j * CG;
+          if constexpr (TYPE == 0) w[j] = __builtin_bit_cast(unsigned, *p);
+          else w[j] = __builtin_bit_cast(unsigned short, *p);
         }
       }
       if constexpr (TYPE == 0) return make_uint4(w[0], w[1], w[2], w[3]);
       else return make_uint2((w[0] & 0xffffu) | (w[1] << 16), (w[2] & 0xffffu) | (w[3] << 16));
     }
   }
-  __device__ __forceinline__ void store(T* row, const float* v) const {
+  __device__ __forceinline__ void store(char* row, unsigned off, const float* v) const {
     if constexpr (WIDE) {
-      if (d0 < D) *reinterpret_cast<W*>(row + d0) = pack<TYPE>(v);
+      if (d0 < D) *reinterpret_cast<W*>(row + off) = pack<TYPE>(v);
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (has(j)) row[channel(j)] = (T)v[j];
+        if (has(j)) (reinterpret_cast<T*>(row + off))[j * CG] = (T)v[j];
     }
   }
-  __device__ __forceinline__ void load_state(const float* s, float* v) const {  // s: channel 0 of a row of fp32 states
+  __device__ __forceinline__ void load_state(const float* s, float* v) const {  // s: the tile's first channel in a row of fp32 states
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = has(j) ? s[channel(j)] : 0.f;
   }
@@ -115,41 +115,40 @@ struct Place {
   }
 };
 
-// f = sigmoid(g) and i = 1 - f = sigmoid(-g), each to a few ulp of itself: e = exp(-g) = 2^p 2^t with p = -g log2(e) rounded and t what the rounding
-// left, f = 1 / (1 + e), i = e f.  Beyond +-104 / -87 both are constant in fp32; NaN passes.
+// a value that is the same in every lane, in a scalar register
+__device__ __forceinline__ unsigned uniform(unsigned v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// f = sigmoid(g) and i = 1 - f = sigmoid(-g), each accurate in itself: e = exp(-|g|), the smaller of the two is e / (1 + e), the larger 1 minus that, with
+// one rounding -- a gate close to one is multiplied with itself over a whole memory, where the error of a reciprocal would add up.  fp32 gates correct
+// exp for what rounding p = -|g| log2(e) has lost, up to |g| 2^-25 of e; 16-bit gates are themselves rounded by more than that.  NaN passes.
+template <int TYPE>
 __device__ __forceinline__ void gate_of(float g, float& f, float& i) {
-  g = g < -87.f ? -87.f : g;
-  g = g > 104.f ? 104.f : g;
-  const float p = g * -1.44269502162933349609375f;
-  float t = fmaf(g, -1.44269502162933349609375f, -p);
-  t = fmaf(g, -1.925963033500011e-08f, t);
-  float e = __builtin_amdgcn_exp2f(p);
-  e = fmaf(e, t * 0.6931471805599453f, e);
-  f = __builtin_amdgcn_rcpf(1.0f + e);
-  i = e * f;
+  float e, m = fabsf(g);
+  if constexpr (TYPE == 0) {
+    m = m > 104.f ? 104.f : m;  // (exp is zero from there on; an infinite one would leave inf - inf below)
+    const float p = m * -1.44269502162933349609375f;
+    float t = fmaf(m, -1.44269502162933349609375f, -p);
+    t = fmaf(m, -1.925963033500011e-08f, t);
+    e = __builtin_amdgcn_exp2f(p);
+    e = fmaf(e, t * 0.6931471805599453f, e);
+  } else {
+    e = __builtin_amdgcn_exp2f(m * -1.44269502162933349609375f);
+  }
+  const float small = e * __builtin_amdgcn_rcpf(1.0f + e), large = 1.0f - small;
+  f = g < 0.f ? small : large;
+  i = g < 0.f ? large : small;
 }
 
-__device__ __forceinline__ unsigned word_of(float v) {
-  const unsigned u = __float_as_uint(v);
-  return u == EMPTY ? 0x7fc00000u : u;
-}
-__device__ __forceinline__ void publish_map(unsigned long long* at, float p, float q) {
-  __hip_atomic_store(at, (unsigned long long)word_of(q) << 32 | word_of(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void publish_state(unsigned* at, float h) { __hip_atomic_store(at, word_of(h), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ unsigned long long peek(const unsigned long long* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ unsigned peek(const unsigned* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
+typedef unsigned long long u64;
 struct ScanArgs {
   vmm_gated_scan_desc d;
-  unsigned* counter;             // the next tile
-  unsigned long long* maps;      // [tile along time][B][D]
-  unsigned* states;              // [group][B][D]
-  int tiles;                     // channel tiles
-  unsigned chunks, total;        // tiles along time, and in all
+  int tiles;           // of 64 channels
+  unsigned units, groups;
+  float2* maps;        // [unit][B][D]; units and groups count in the direction of the walk
+  float2* group_maps;  // [group][B][D]
+  float* anchors;      // [group / 256][B][D]
+  float* states;       // [unit][B][D]: the state in front of each (forward: the caller's, where it keeps them)
 };
-
-constexpr int GROUP = 16;
 
 // the map of the segments before (FORWARD) or behind this one inside its wave, and the wave's own map, from the segment's (p, q)
 template <bool FORWARD>
@@ -162,10 +161,8 @@ __device__ __forceinline__ void wave_join(float* p, float* q, float* pe, float* 
       const bool upper = threadIdx.x & (1u << bit);
       const bool later = upper == FORWARD;  // this side's map is applied after the other's
       const float pp = lane_xor(p[j], bit), qq = lane_xor(q[j], bit);
-      if (later) {  // (its exclusive part follows everything of the other side)
-        qe[j] = fmaf(pe[j], qq, qe[j]);
-        pe[j] *= pp;
-      }
+      qe[j] = later ? fmaf(pe[j], qq, qe[j]) : qe[j];  // (its exclusive part follows everything of the other side)
+      pe[j] = later ? pe[j] * pp : pe[j];
       const float first_q = later ? qq : q[j], then_p = later ? p[j] : pp, then_q = later ? q[j] : qq;
       q[j] = fmaf(then_p, first_q, then_q);
       p[j] *= pp;
@@ -173,378 +170,436 @@ __device__ __forceinline__ void wave_join(float* p, float* q, float* pe, float* 
   }
 }
 
-// The state in front of tile `c` (c counts in the direction of the walk), from the state at its group's start and the maps since.
-// Sixteen rows of lanes fetch one map each, so the waits for a group's maps are one wait; joined by every wave for itself.
-template <int TYPE, bool WIDE>
-__device__ __forceinline__ void carry_in(const ScanArgs& a, const Place<TYPE, WIDE>& at, unsigned c, int b, const float* start, float (*got)[CG][2 * V],
-                                         float* h) {
-  const int cg = threadIdx.x & 15, row = threadIdx.x >> 4;
-  const unsigned base = c / GROUP * GROUP, mine = base + row;
-  const long long BD = (long long)a.d.B * a.d.D, bd = (long long)b * a.d.D;
-  if (mine < c) {
-    const unsigned long long* m = a.maps + mine * BD + bd;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      unsigned long long w = 0;
-      if (at.has(j)) {
-        while ((unsigned)(w = peek(m + at.channel(j))) == EMPTY) __builtin_amdgcn_s_sleep(1);
-      }
-      got[row][cg][2 * j] = __uint_as_float((unsigned)w);
-      got[row][cg][2 * j + 1] = __uint_as_float((unsigned)(w >> 32));
-    }
-  } else if (row == GROUP - 1) {  // c - base is 15 at most: this row has no map to fetch
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float v = start[j];
-      if (base > 0 && at.has(j)) {
-        const unsigned* s = a.states + (base / GROUP - 1) * BD + bd + at.channel(j);
-        unsigned w;
-        while ((w = peek(s)) == EMPTY) __builtin_amdgcn_s_sleep(1);
-        v = __uint_as_float(w);
-      }
-      got[row][cg][j] = v;
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < V; ++j) h[j] = got[GROUP - 1][cg][j];
-  for (unsigned k = 0; k < c - base; ++k)
-#pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = fmaf(got[k][cg][2 * j], h[j], got[k][cg][2 * j + 1]);
-}
-
-template <int TYPE, bool WIDE, int TS>
-__global__ __launch_bounds__(256, 3) void scan_fwd_kernel(const ScanArgs a) {
-  typedef typename Elem<TYPE>::T T;
-  constexpr int TILE = 16 * TS;
-  __shared__ float wave_map[4][CG][2 * V];
-  __shared__ float got[16][CG][2 * V];
-  __shared__ unsigned next_tile;
+// ---- step 1.  A workgroup makes the maps of a group: a wave a unit, a lane 4 channels and a quarter of its steps, eight (fp32: four) at a time with the
+// next ones on their way.  Forward from x and gate, BACK from dy and gate.
+template <int TYPE, bool WIDE, bool BACK>
+__global__ __launch_bounds__(1024) void scan_map_kernel(const ScanArgs a) {
+  constexpr int STEPS = UNIT / 4, BATCH = TYPE == 0 ? 4 : 8, BATCHES = STEPS / BATCH;
+  __shared__ float2 join[GROUP][CG][V];
   const vmm_gated_scan_desc& d = a.d;
-  const int cg = threadIdx.x & 15, seg = threadIdx.x >> 4, wave = threadIdx.x >> 6;
-  const long long BD = (long long)d.B * d.D;
-  unsigned tile = blockIdx.x;
-  if (a.chunks > 1) {
-    if (threadIdx.x == 0) next_tile = atomicAdd(a.counter, 1u);
-    __syncthreads();
-    tile = next_tile;
-  }
-  while (tile < a.total) {
-    const unsigned per = (unsigned)d.B * a.tiles;
-    const unsigned c = tile / per, bt = tile % per;
-    const int b = bt / a.tiles;
-    const Place<TYPE, WIDE> at(bt % a.tiles, cg, d.D);
-    const long long len = d.lengths ? max(0LL, min((long long)d.lengths[b], (long long)d.L)) : (long long)d.L;
-    const long long t0 = (long long)c * TILE + seg * TS;
-    const T* xr = (const T*)d.x + b * d.x_batch + t0 * d.x_row;
-    const T* gr = (const T*)d.gate + b * d.gate_batch + t0 * d.gate_row;
-    Raw<TYPE> x[TS], g[TS];
-    if (t0 + TS <= len) {
+  const int cg = threadIdx.x & 15, quarter = (threadIdx.x >> 4) & 3, wave = uniform(threadIdx.x >> 6);
+  const unsigned tile = blockIdx.x % a.tiles, rest = uniform(blockIdx.x / a.tiles), group = uniform(rest / d.B), b = rest - group * d.B;
+  const Place<TYPE, WIDE> at(cg, d.D - (int)tile * CG * V);
+  const unsigned u = group * GROUP + wave;  // in the direction of the walk
+  const bool exists = u < a.units;
+  const long long first = (long long)(BACK ? a.units - 1 - u : u) * UNIT;
+  long long len = d.L;
+  if (d.lengths) len = max(0LL, min((long long)d.lengths[b], len));
+  const int live = exists ? (int)min(max(len - first, 0LL), (long long)UNIT) - quarter * STEPS : 0;
+  const long long es = sizeof(typename Elem<TYPE>::T), bd = (long long)b * d.D + (long long)tile * CG * V;
+  const void* xv = BACK ? d.dy : d.x;
+  const int64_t xb = BACK ? d.dy_batch : d.x_batch, xs = BACK ? d.dy_row : d.x_row;
+  const auto row = [&](const void* p, int64_t batch, int64_t step, int k) {
+    return (const char*)p + (b * batch + (first + k) * step + (long long)tile * CG * V) * es;
+  };
+  const unsigned xl = (quarter * STEPS * (unsigned)xs + at.d0) * (unsigned)es, gl = (quarter * STEPS * (unsigned)d.gate_row + at.d0) * (unsigned)es;
+  const bool has_x = !BACK || d.dy;
+  Raw<TYPE> x[BATCH], g[BATCH];
+  auto load = [&](int k0) {
 #pragma unroll
-      for (int k = 0; k < TS; ++k) { x[k].u = at.load(xr + k * d.x_row, 0u); g[k].u = at.load(gr + k * d.gate_row, Elem<TYPE>::PAD); }
-    } else {
-#pragma unroll
-      for (int k = 0; k < TS; ++k) {
-        x[k].u = fill_word<TYPE>(0u);
-        g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
-        if (t0 + k < len) { x[k].u = at.load(xr + k * d.x_row, 0u); g[k].u = at.load(gr + k * d.gate_row, Elem<TYPE>::PAD); }
+    for (int k = 0; k < BATCH; ++k) {
+      x[k].u = fill_word<TYPE>(0u);
+      g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
+      if (k0 + k < live) {
+        if (has_x) x[k].u = at.load(row(xv, xb, xs, k0 + k), xl, 0u);
+        g[k].u = at.load(row(d.gate, d.gate_batch, d.gate_row, k0 + k), gl, Elem<TYPE>::PAD);
       }
     }
-    unsigned ahead = 0;
-    if (a.chunks > 1 && threadIdx.x == 0) ahead = atomicAdd(a.counter, 1u);
-    float start[V];
+  };
+  float P[V], Q[V], pe[V], qe[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) start[j] = 0.f;
-    if (c < GROUP && d.h0) at.load_state(d.h0 + (long long)b * d.D, start);
-
-    float f[TS][V], q[TS][V], P[V], Q[V], pe[V], qe[V];
+  for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; }
+  load(BACK ? STEPS - BATCH : 0);
 #pragma unroll
-    for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; }
+  for (int n = 0; n < BATCHES; ++n) {
+    float f[BATCH][V], q[BATCH][V];
 #pragma unroll
-    for (int k = 0; k < TS; ++k)
+    for (int k = 0; k < BATCH; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         float i;
-        gate_of(g[k].get(j), f[k][j], i);
-        q[k][j] = i * x[k].get(j);
+        gate_of<TYPE>(g[k].get(j), f[k][j], i);
+        q[k][j] = BACK ? x[k].get(j) : i * x[k].get(j);
+      }
+    if (n + 1 < BATCHES) load((BACK ? BATCHES - 2 - n : n + 1) * BATCH);
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) {
+      const int k = BACK ? BATCH - 1 - s : s;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        Q[j] = BACK ? f[k][j] * (q[k][j] + Q[j]) : fmaf(f[k][j], Q[j], q[k][j]);
         P[j] *= f[k][j];
-        Q[j] = fmaf(f[k][j], Q[j], q[k][j]);
-      }
-    wave_join<true>(P, Q, pe, qe);
-    if ((threadIdx.x & 48) == 0) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) { wave_map[wave][cg][2 * j] = P[j]; wave_map[wave][cg][2 * j + 1] = Q[j]; }
-    }
-    __syncthreads();
-    float pw[V], qw[V];  // the waves before this one
-#pragma unroll
-    for (int j = 0; j < V; ++j) { pw[j] = 1.f; qw[j] = 0.f; }
-    for (int w = 0; w < wave; ++w)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float p1 = wave_map[w][cg][2 * j], q1 = wave_map[w][cg][2 * j + 1];
-        pw[j] *= p1;
-        qw[j] = fmaf(p1, qw[j], q1);
-      }
-    if (a.chunks > 1) {
-      if (threadIdx.x == 0) next_tile = ahead;
-      if (seg == 15 && c + 1 < a.chunks && c % GROUP != GROUP - 1) {
-        unsigned long long* m = a.maps + c * BD + (long long)b * d.D;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (at.has(j)) publish_map(m + at.channel(j), P[j] * pw[j], fmaf(P[j], qw[j], Q[j]));
-      }
-      carry_in<TYPE, WIDE>(a, at, c, b, start, got, start);
-    }
-    float h[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = fmaf(pe[j], fmaf(pw[j], start[j], qw[j]), qe[j]);
-    if (d.states && (seg * TS) % STATE_STEP == 0) {
-      const long long s = (long long)c * (TILE / STATE_STEP) + seg * TS / STATE_STEP;
-      if (s * STATE_STEP < d.L) at.store_state(d.states + s * BD + (long long)b * d.D, h);
-    }
-    T* yr = (T*)d.y + b * d.y_batch + t0 * d.y_row;
-#pragma unroll
-    for (int k = 0; k < TS; ++k) {
-      float o[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        h[j] = fmaf(f[k][j], h[j], q[k][j]);
-        o[j] = t0 + k < len ? h[j] : 0.f;
-      }
-      if (t0 + k < d.L) at.store(yr + k * d.y_row, o);
-    }
-    if (seg == 15) {
-      if (c + 1 == a.chunks) {
-        if (d.h_last) at.store_state(d.h_last + (long long)b * d.D, h);
-      } else if (c % GROUP == GROUP - 1) {
-        unsigned* s = a.states + c / GROUP * BD + (long long)b * d.D;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (at.has(j)) publish_state(s + at.channel(j), h[j]);
       }
     }
-    if (a.chunks == 1) break;
-    tile = next_tile;  // (written before carry_in's barrier; written again behind the next tile's first one)
+  }
+  wave_join<!BACK>(P, Q, pe, qe);
+  if (quarter == 0) {
+    float2* m = a.maps + (long long)u * d.B * d.D + bd;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      join[wave][cg][j] = make_float2(P[j], Q[j]);
+      if (exists && at.has(j)) m[at.channel(j)] = make_float2(P[j], Q[j]);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    float2* gm = a.group_maps + (long long)group * d.B * d.D + bd;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float p = 1.f, q = 0.f;
+      for (int r = 0; r < GROUP; ++r) {  // (units that do not exist left the identity)
+        const float2 w = join[r][cg][j];
+        p *= w.x;
+        q = fmaf(w.x, q, w.y);
+      }
+      if (at.has(j)) gm[at.channel(j)] = make_float2(p, q);
+    }
   }
 }
 
-template <int TYPE, bool WIDE, int TS>
+// ---- step 2.  16 lanes of 4 channels x 16 rows a workgroup, as above; channels side by side (maps and states are the kernels' own: always aligned to
+// their type, which is all that is asked for here).
+
+// h = the maps [from, to) applied to h: each row joins a sixteenth of them, and every row then applies the sixteen
+__device__ __forceinline__ void apply_range(const float2* maps, long long BD, unsigned from, unsigned to, const bool* has, const int* channel, float2 (*join)[CG][V],
+                                            float* h) {
+  const int cg = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const unsigned n = to - from, r0 = from + n * row / 16, r1 = from + n * (row + 1) / 16;
+  float p[V], q[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) { p[j] = 1.f; q[j] = 0.f; }
+#pragma unroll 4
+  for (unsigned r = r0; r < r1; ++r)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 w = has[j] ? maps[r * BD + channel[j]] : make_float2(1.f, 0.f);
+      p[j] *= w.x;
+      q[j] = fmaf(w.x, q[j], w.y);
+    }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < V; ++j) join[row][cg][j] = make_float2(p[j], q[j]);
+  __syncthreads();
+  for (int r = 0; r < 16; ++r)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 w = join[r][cg][j];
+      h[j] = fmaf(w.x, h[j], w.y);
+    }
+}
+
+__global__ __launch_bounds__(256) void scan_anchor_kernel(const ScanArgs a, const float* start) {
+  __shared__ float2 join[16][CG][V];
+  const int cg = threadIdx.x & 15, row = threadIdx.x >> 4, tile = blockIdx.x % a.tiles, b = blockIdx.x / a.tiles;
+  const long long BD = (long long)a.d.B * a.d.D, bd = (long long)b * a.d.D;
+  bool has[V];
+  int channel[V];
+  float h[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    channel[j] = (tile * CG + cg) * V + j;
+    has[j] = channel[j] < a.d.D;
+    h[j] = start && has[j] ? start[bd + channel[j]] : 0.f;
+  }
+  for (unsigned k = 1; k * ANCHOR < a.groups; ++k) {
+    apply_range(a.group_maps + bd, BD, (k - 1) * ANCHOR, k * ANCHOR, has, channel, join, h);
+    if (row == 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (has[j]) a.anchors[(k - 1) * BD + bd + channel[j]] = h[j];
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void scan_states_kernel(const ScanArgs a, const float* start) {
+  __shared__ float2 join[16][CG][V];
+  const int cg = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const unsigned tile = blockIdx.x % a.tiles, rest = blockIdx.x / a.tiles, b = rest % a.d.B, group = rest / a.d.B, anchor = group / ANCHOR;
+  const long long BD = (long long)a.d.B * a.d.D, bd = (long long)b * a.d.D;
+  const unsigned u = group * GROUP + row;
+  bool has[V];
+  int channel[V];
+  float h[V];
+  float2 own[V];
+  const float* from = anchor ? a.anchors + (anchor - 1) * BD : start;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    channel[j] = (tile * CG + cg) * V + j;
+    has[j] = channel[j] < (unsigned)a.d.D;
+    h[j] = from && has[j] ? from[bd + channel[j]] : 0.f;
+    own[j] = u < a.units && has[j] ? a.maps[u * BD + bd + channel[j]] : make_float2(1.f, 0.f);
+  }
+  apply_range(a.group_maps + bd, BD, anchor * ANCHOR, group, has, channel, join, h);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < V; ++j) join[row][cg][j] = own[j];
+  __syncthreads();
+  for (int r = 0; r < row; ++r)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 w = join[r][cg][j];
+      h[j] = fmaf(w.x, h[j], w.y);
+    }
+  if (u < a.units) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (has[j]) a.states[u * BD + bd + channel[j]] = h[j];
+  }
+}
+
+// ---- step 3.  A workgroup takes a unit into registers: 16 segments of 4 steps, joined with lane exchanges inside a wave and through LDS between the four
+// waves, so that a short sequence does not wait step by step.
+template <int TYPE, bool WIDE>
+__global__ __launch_bounds__(256, 4) void scan_fwd_kernel(const ScanArgs a) {
+  constexpr int TS = UNIT / 16;
+  __shared__ float2 wave_map[4][CG][V];
+  const vmm_gated_scan_desc& d = a.d;
+  const int cg = threadIdx.x & 15, seg = threadIdx.x >> 4, wave = threadIdx.x >> 6;
+  const unsigned tile = blockIdx.x % a.tiles, rest = uniform(blockIdx.x / a.tiles), turn = uniform(rest / d.B), b = rest - turn * d.B;
+  const unsigned u = a.units - 1 - turn;  // from the end of time, where the maps were read last
+  const long long first = (long long)u * UNIT;
+  const Place<TYPE, WIDE> at(cg, d.D - (int)tile * CG * V);
+  long long len = d.L;
+  if (d.lengths) len = max(0LL, min((long long)d.lengths[b], len));
+  const int live = (int)min(max(len - first, 0LL), (long long)UNIT) - seg * TS, there = (int)min(d.L - first, (int64_t)UNIT) - seg * TS;
+  const long long es = sizeof(typename Elem<TYPE>::T), bd = (long long)b * d.D + (long long)tile * CG * V;
+  const auto row = [&](auto* p, int64_t batch, int64_t step, int k) { return p + (b * batch + (first + k) * step + (long long)tile * CG * V) * es; };
+  const auto lane = [&](int64_t step) { return (seg * TS * (unsigned)step + at.d0) * (unsigned)es; };
+  Raw<TYPE> x[TS], g[TS];
+  const unsigned xl = lane(d.x_row), gl = lane(d.gate_row);
+#pragma unroll
+  for (int k = 0; k < TS; ++k) {
+    x[k].u = fill_word<TYPE>(0u);
+    g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
+    if (k < live) {
+      x[k].u = at.load(row((const char*)d.x, d.x_batch, d.x_row, k), xl, 0u);
+      g[k].u = at.load(row((const char*)d.gate, d.gate_batch, d.gate_row, k), gl, Elem<TYPE>::PAD);
+    }
+  }
+  float h[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) h[j] = 0.f;
+  if (a.units > 1) at.load_state(a.states + (long long)u * d.B * d.D + bd, h);
+  else if (d.h0) at.load_state(d.h0 + bd, h);
+  if (a.units == 1 && d.states && seg == 0) at.store_state(d.states + bd, h);  // (step 2 would have left it)
+
+  float f[TS][V], q[TS][V], P[V], Q[V], pe[V], qe[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; }
+#pragma unroll
+  for (int k = 0; k < TS; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float i;
+      gate_of<TYPE>(g[k].get(j), f[k][j], i);
+      q[k][j] = i * x[k].get(j);
+      P[j] *= f[k][j];
+      Q[j] = fmaf(f[k][j], Q[j], q[k][j]);
+    }
+  wave_join<true>(P, Q, pe, qe);
+  if ((threadIdx.x & 48) == 0) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) wave_map[wave][cg][j] = make_float2(P[j], Q[j]);
+  }
+  __syncthreads();  // (and every wave has read h0, which h_last may be)
+  for (int w = 0; w < wave; ++w)
+#pragma unroll
+    for (int j = 0; j < V; ++j) h[j] = fmaf(wave_map[w][cg][j].x, h[j], wave_map[w][cg][j].y);
+#pragma unroll
+  for (int j = 0; j < V; ++j) h[j] = fmaf(pe[j], h[j], qe[j]);
+  const unsigned yl = lane(d.y_row);
+#pragma unroll
+  for (int k = 0; k < TS; ++k) {
+    float o[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      h[j] = fmaf(f[k][j], h[j], q[k][j]);
+      o[j] = k < live ? h[j] : 0.f;
+    }
+    if (k < there) at.store(row((char*)d.y, d.y_batch, d.y_row, k), yl, o);
+  }
+  if (seg == 15 && u + 1 == a.units && d.h_last) at.store_state(d.h_last + bd, h);
+}
+
+// backward: h has to be known forwards and c backwards, so the segments are joined in both directions
+template <int TYPE, bool WIDE>
 __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(const ScanArgs a) {
-  typedef typename Elem<TYPE>::T T;
-  constexpr int TILE = 16 * TS;
-  static_assert(TILE == STATE_STEP, "a tile starts from the state that the forward kept");
+  constexpr int TS = UNIT / 16;
   __shared__ float wave_map[2][4][CG][2 * V];
-  __shared__ float got[16][CG][2 * V];
-  __shared__ unsigned next_tile;
   const vmm_gated_scan_desc& d = a.d;
   const int cg = threadIdx.x & 15, seg = threadIdx.x >> 4, wave = threadIdx.x >> 6;
   const long long BD = (long long)d.B * d.D;
-  unsigned tile = blockIdx.x;
-  if (a.chunks > 1) {
-    if (threadIdx.x == 0) next_tile = atomicAdd(a.counter, 1u);
-    __syncthreads();
-    tile = next_tile;
+  const unsigned tile = blockIdx.x % a.tiles, rest = uniform(blockIdx.x / a.tiles), b = rest % d.B;
+  const unsigned u = rest / d.B, v = a.units - 1 - u;  // from the start of time (where the maps were read last), and in the direction of the walk
+  const long long first = (long long)u * UNIT;
+  const Place<TYPE, WIDE> at(cg, d.D - (int)tile * CG * V);
+  long long len = d.L;
+  if (d.lengths) len = max(0LL, min((long long)d.lengths[b], len));
+  const int live = (int)min(max(len - first, 0LL), (long long)UNIT) - seg * TS, there = (int)min(d.L - first, (int64_t)UNIT) - seg * TS;
+  const long long es = sizeof(typename Elem<TYPE>::T), bd = (long long)b * d.D + (long long)tile * CG * V;
+  const auto row = [&](auto* p, int64_t batch, int64_t step, int k) { return p + (b * batch + (first + k) * step + (long long)tile * CG * V) * es; };
+  const auto lane = [&](int64_t step) { return (seg * TS * (unsigned)step + at.d0) * (unsigned)es; };
+  Raw<TYPE> x[TS], g[TS], dy[TS];
+  const unsigned xl = lane(d.x_row), gl = lane(d.gate_row), yl = lane(d.dy_row);
+#pragma unroll
+  for (int k = 0; k < TS; ++k) {
+    x[k].u = dy[k].u = fill_word<TYPE>(0u);
+    g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
+    if (k < live) {
+      x[k].u = at.load(row((const char*)d.x, d.x_batch, d.x_row, k), xl, 0u);
+      g[k].u = at.load(row((const char*)d.gate, d.gate_batch, d.gate_row, k), gl, Elem<TYPE>::PAD);
+      if (d.dy) dy[k].u = at.load(row((const char*)d.dy, d.dy_batch, d.dy_row, k), yl, 0u);
+    }
   }
-  while (tile < a.total) {
-    const unsigned per = (unsigned)d.B * a.tiles;
-    const unsigned r = tile / per, bt = tile % per, c = a.chunks - 1 - r;  // r counts from the end of time
-    const int b = bt / a.tiles;
-    const long long bd = (long long)b * d.D;
-    const Place<TYPE, WIDE> at(bt % a.tiles, cg, d.D);
-    const long long len = d.lengths ? max(0LL, min((long long)d.lengths[b], (long long)d.L)) : (long long)d.L;
-    const long long t0 = (long long)c * TILE + seg * TS;
-    const T* xr = (const T*)d.x + b * d.x_batch + t0 * d.x_row;
-    const T* gr = (const T*)d.gate + b * d.gate_batch + t0 * d.gate_row;
-    const T* yr = (const T*)d.dy + b * d.dy_batch + t0 * d.dy_row;
-    Raw<TYPE> x[TS], g[TS], dy[TS];
+  float h[V], back[V];
+  at.load_state(d.states + u * BD + bd, h);
 #pragma unroll
-    for (int k = 0; k < TS; ++k) {
-      x[k].u = dy[k].u = fill_word<TYPE>(0u);
-      g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
-      if (t0 + k < len) {
-        x[k].u = at.load(xr + k * d.x_row, 0u);
-        g[k].u = at.load(gr + k * d.gate_row, Elem<TYPE>::PAD);
-        if (d.dy) dy[k].u = at.load(yr + k * d.dy_row, 0u);
-      }
-    }
-    unsigned ahead = 0;
-    if (a.chunks > 1 && threadIdx.x == 0) ahead = atomicAdd(a.counter, 1u);
-    float h[V], start[V];
-    at.load_state(d.states + c * BD + bd, h);
-#pragma unroll
-    for (int j = 0; j < V; ++j) start[j] = 0.f;
-    if (r < GROUP && d.dh_last) at.load_state(d.dh_last + bd, start);
+  for (int j = 0; j < V; ++j) back[j] = 0.f;
+  if (a.units > 1) at.load_state(a.states + v * BD + bd, back);
+  else if (d.dh_last) at.load_state(d.dh_last + bd, back);
 
-    float f[TS][V], i[TS][V], P[V], Q[V], R[V], pf[V], qf[V], pb[V], rb[V], P2[V];
+  float f[TS][V], i[TS][V], P[V], Q[V], R[V], pf[V], qf[V], pb[V], rb[V], P2[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; R[j] = 0.f; }
+  for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; R[j] = 0.f; }
 #pragma unroll
-    for (int k = 0; k < TS; ++k)
+  for (int k = 0; k < TS; ++k)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        gate_of(g[k].get(j), f[k][j], i[k][j]);
-        P[j] *= f[k][j];
-        Q[j] = fmaf(f[k][j], Q[j], i[k][j] * x[k].get(j));
-      }
-#pragma unroll
-    for (int k = TS - 1; k >= 0; --k)
-#pragma unroll
-      for (int j = 0; j < V; ++j) R[j] = f[k][j] * (dy[k].get(j) + R[j]);
-#pragma unroll
-    for (int j = 0; j < V; ++j) P2[j] = P[j];
-    wave_join<true>(P, Q, pf, qf);
-    wave_join<false>(P2, R, pb, rb);
-    if ((threadIdx.x & 48) == 0) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        wave_map[0][wave][cg][2 * j] = P[j]; wave_map[0][wave][cg][2 * j + 1] = Q[j];
-        wave_map[1][wave][cg][2 * j] = P2[j]; wave_map[1][wave][cg][2 * j + 1] = R[j];
-      }
+    for (int j = 0; j < V; ++j) {
+      gate_of<TYPE>(g[k].get(j), f[k][j], i[k][j]);
+      P[j] *= f[k][j];
+      Q[j] = fmaf(f[k][j], Q[j], i[k][j] * x[k].get(j));
     }
-    __syncthreads();
-    for (int w = 0; w < wave; ++w)  // the state in front of this wave
 #pragma unroll
-      for (int j = 0; j < V; ++j) h[j] = fmaf(wave_map[0][w][cg][2 * j], h[j], wave_map[0][w][cg][2 * j + 1]);
+  for (int k = TS - 1; k >= 0; --k)
 #pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = fmaf(pf[j], h[j], qf[j]);
-    float pw[V], rw[V];  // the waves behind this one
+    for (int j = 0; j < V; ++j) R[j] = f[k][j] * (dy[k].get(j) + R[j]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) { pw[j] = 1.f; rw[j] = 0.f; }
-    for (int w = 3; w > wave; --w)
+  for (int j = 0; j < V; ++j) P2[j] = P[j];
+  wave_join<true>(P, Q, pf, qf);
+  wave_join<false>(P2, R, pb, rb);
+  if ((threadIdx.x & 48) == 0) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float p1 = wave_map[1][w][cg][2 * j], r1 = wave_map[1][w][cg][2 * j + 1];
-        pw[j] *= p1;
-        rw[j] = fmaf(p1, rw[j], r1);
-      }
-    if (a.chunks > 1) {
-      if (threadIdx.x == 0) next_tile = ahead;
-      if (seg == 0 && r + 1 < a.chunks && r % GROUP != GROUP - 1) {
-        unsigned long long* m = a.maps + r * BD + bd;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (at.has(j)) publish_map(m + at.channel(j), P2[j] * pw[j], fmaf(P2[j], rw[j], R[j]));
-      }
-      carry_in<TYPE, WIDE>(a, at, r, b, start, got, start);
+    for (int j = 0; j < V; ++j) {
+      wave_map[0][wave][cg][2 * j] = P[j]; wave_map[0][wave][cg][2 * j + 1] = Q[j];
+      wave_map[1][wave][cg][2 * j] = P2[j]; wave_map[1][wave][cg][2 * j + 1] = R[j];
     }
-    float back[V];  // c_(t+1) of the segment's last step
-#pragma unroll
-    for (int j = 0; j < V; ++j) back[j] = fmaf(pb[j], fmaf(pw[j], start[j], rw[j]), rb[j]);
-    // h_(t-1) - x_t, forwards; it takes the place of x
-    float hx[TS][V];
-#pragma unroll
-    for (int k = 0; k < TS; ++k)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float xv = x[k].get(j);
-        hx[k][j] = h[j] - xv;
-        h[j] = fmaf(f[k][j], h[j], i[k][j] * xv);
-      }
-    T* xo = (T*)d.dx + b * d.dx_batch + t0 * d.dx_row;
-    T* go = (T*)d.dgate + b * d.dgate_batch + t0 * d.dgate_row;
-#pragma unroll
-    for (int k = TS - 1; k >= 0; --k) {
-      float ox[V], og[V];
-      const bool live = t0 + k < len;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float dh = dy[k].get(j) + back[j], di = dh * i[k][j];
-        ox[j] = live ? di : 0.f;
-        og[j] = live ? di * f[k][j] * hx[k][j] : 0.f;
-        back[j] = f[k][j] * dh;
-      }
-      if (t0 + k < d.L) {
-        if (d.dx) at.store(xo + k * d.dx_row, ox);
-        if (d.dgate) at.store(go + k * d.dgate_row, og);
-      }
-    }
-    if (seg == 0) {
-      if (c == 0) {
-        if (d.dh0) at.store_state(d.dh0 + bd, back);
-      } else if (r % GROUP == GROUP - 1) {
-        unsigned* s = a.states + r / GROUP * BD + bd;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (at.has(j)) publish_state(s + at.channel(j), back[j]);
-      }
-    }
-    if (a.chunks == 1) break;
-    tile = next_tile;
   }
+  __syncthreads();
+  for (int w = 0; w < wave; ++w)  // the state in front of this wave
+#pragma unroll
+    for (int j = 0; j < V; ++j) h[j] = fmaf(wave_map[0][w][cg][2 * j], h[j], wave_map[0][w][cg][2 * j + 1]);
+  for (int w = 3; w > wave; --w)  // and what the waves behind it hand on
+#pragma unroll
+    for (int j = 0; j < V; ++j) back[j] = fmaf(wave_map[1][w][cg][2 * j], back[j], wave_map[1][w][cg][2 * j + 1]);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    h[j] = fmaf(pf[j], h[j], qf[j]);
+    back[j] = fmaf(pb[j], back[j], rb[j]);  // c_(t+1) of the segment's last step
+  }
+  float hx[TS][V];  // h_(t-1) - x_t, forwards
+#pragma unroll
+  for (int k = 0; k < TS; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float xv = x[k].get(j);
+      hx[k][j] = h[j] - xv;
+      h[j] = fmaf(f[k][j], h[j], i[k][j] * xv);
+    }
+  const unsigned xo = lane(d.dx_row), go = lane(d.dgate_row);
+#pragma unroll
+  for (int k = TS - 1; k >= 0; --k) {
+    float ox[V], og[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float dh = dy[k].get(j) + back[j], di = dh * i[k][j];
+      ox[j] = k < live ? di : 0.f;
+      og[j] = k < live ? di * f[k][j] * hx[k][j] : 0.f;
+      back[j] = f[k][j] * dh;
+    }
+    if (k < there) {
+      if (d.dx) at.store(row((char*)d.dx, d.dx_batch, d.dx_row, k), xo, ox);
+      if (d.dgate) at.store(row((char*)d.dgate, d.dgate_batch, d.dgate_row, k), go, og);
+    }
+  }
+  if (seg == 0 && u == 0 && d.dh0) at.store_state(d.dh0 + bd, back);
 }
-
-__global__ __launch_bounds__(256) void scan_clear_kernel(unsigned* counter, uint4* p, long long n) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i == 0) *counter = 0u;
-  if (i < n) p[i] = make_uint4(EMPTY, EMPTY, EMPTY, EMPTY);
-}
-
-constexpr int FWD_TS = 8, BWD_TS = 4;
 
 inline int esize(int type) { return type == 0 ? 4 : 2; }
+inline long long up16(long long n) { return (n + 15) / 16 * 16; }
 
+bool bad_rows(int64_t row) { return row < 0 || row >= (1LL << 23); }  // 64 rows are addressed with 32-bit byte offsets
 bool bad_scan(const vmm_gated_scan_desc* d) {
-  return !d || d->B < 0 || d->D < 0 || d->L < 0 || d->L >= (1LL << 31) || d->type < 0 || d->type > 2 || (int64_t)d->B * d->D >= (1LL << 31);
+  return !d || d->B < 0 || d->D < 0 || d->L < 0 || d->L >= (1LL << 31) || d->type < 0 || d->type > 2 || (int64_t)d->B * d->D >= (1LL << 31) ||
+         bad_rows(d->x_row) || bad_rows(d->gate_row) || bad_rows(d->y_row) || bad_rows(d->dy_row) || bad_rows(d->dx_row) || bad_rows(d->dgate_row);
 }
-struct Layout { unsigned chunks; long long maps, states; };  // counts of words
+
+struct Layout { unsigned units, groups; long long group_maps, anchors, states, bytes; };
 Layout layout(const vmm_gated_scan_desc* d, bool backward) {
-  const int tile = 16 * (backward ? BWD_TS : FWD_TS);
-  Layout l;
-  l.chunks = (unsigned)((d->L + tile - 1) / tile);
+  Layout l = {};
+  l.units = (unsigned)((d->L + UNIT - 1) / UNIT);
+  l.groups = (l.units + GROUP - 1) / GROUP;
+  if (l.units < 2) return l;
   const long long BD = (long long)d->B * d->D;
-  l.maps = l.chunks > 1 ? l.chunks * BD : 0;
-  l.states = l.chunks > 1 ? (l.chunks / GROUP + 1) * BD : 0;
+  l.group_maps = up16(8 * BD * l.units);
+  l.anchors = l.group_maps + up16(8 * BD * l.groups);
+  l.states = l.anchors + up16(4 * BD * ((l.groups - 1) / ANCHOR));
+  l.bytes = l.states + (backward || !d->states ? up16(4 * BD * l.units) : 0);
   return l;
 }
-inline long long up16(long long n) { return (n + 15) / 16 * 16; }
 
 // accesses of four values to rows of D: addresses, strides and D itself have to allow them
 bool wide(const void* p, int64_t batch, int64_t row, int D, int type) {
   return !p || (((uintptr_t)p & (V * esize(type) - 1)) == 0 && batch % V == 0 && row % V == 0 && D % V == 0);
 }
 
-template <bool FWD, int TYPE>
-void launch(const ScanArgs& a, bool w, int blocks, hipStream_t s) {
-  if constexpr (FWD) {
-    if (w) hipLaunchKernelGGL((scan_fwd_kernel<TYPE, true, FWD_TS>), dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((scan_fwd_kernel<TYPE, false, FWD_TS>), dim3(blocks), dim3(256), 0, s, a);
-  } else {
-    if (w) hipLaunchKernelGGL((scan_bwd_kernel<TYPE, true, BWD_TS>), dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((scan_bwd_kernel<TYPE, false, BWD_TS>), dim3(blocks), dim3(256), 0, s, a);
-  }
-}
-
-template <bool FWD>
-int scan(const vmm_gated_scan_desc* d, hipStream_t s) {
-  const Layout l = layout(d, !FWD);
-  ScanArgs a;
-  a.d = *d;
-  a.tiles = (d->D + CG * V - 1) / (CG * V);
-  a.chunks = l.chunks;
-  const unsigned long long total = (unsigned long long)l.chunks * d->B * a.tiles;
-  if (total >= 0xff000000ull) return -1;  // (the counter runs past it by the number of workgroups)
-  a.total = (unsigned)total;
-  int blocks = (int)total;
-  if (l.chunks > 1) {
-    if (!d->workspace || ((uintptr_t)d->workspace & 15)) return -1;
-    a.counter = (unsigned*)d->workspace;
-    a.maps = (unsigned long long*)((char*)d->workspace + 16);
-    a.states = (unsigned*)((char*)d->workspace + 16 + up16(8 * l.maps));
-    const long long n = (up16(8 * l.maps) + up16(4 * l.states)) / 16;
-    hipLaunchKernelGGL(scan_clear_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a.counter, (uint4*)a.maps, n);
+template <int TYPE, bool WIDE>
+int run(const ScanArgs& a, bool forward, hipStream_t s) {
+  const unsigned chains = (unsigned)a.d.B * a.tiles;
+  if (a.units > 1) {
+    const float* start = forward ? a.d.h0 : a.d.dh_last;
+    const unsigned blocks = chains * a.groups;
+    if (forward) hipLaunchKernelGGL((scan_map_kernel<TYPE, WIDE, false>), dim3(blocks), dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((scan_map_kernel<TYPE, WIDE, true>), dim3(blocks), dim3(1024), 0, s, a);
     VMM_LAUNCH_CHECK();
-    blocks = (int)min(total, 1024ull);  // at least what the card holds at once; each takes tiles until none is left
+    if (a.groups > ANCHOR) {
+      hipLaunchKernelGGL(scan_anchor_kernel, dim3(chains), dim3(256), 0, s, a, start);
+      VMM_LAUNCH_CHECK();
+    }
+    hipLaunchKernelGGL(scan_states_kernel, dim3(blocks), dim3(256), 0, s, a, start);
+    VMM_LAUNCH_CHECK();
   }
-  const bool w = wide(d->x, d->x_batch, d->x_row, d->D, d->type) && wide(d->gate, d->gate_batch, d->gate_row, d->D, d->type) &&
-                 (FWD ? wide(d->y, d->y_batch, d->y_row, d->D, d->type)
-                      : wide(d->dy, d->dy_batch, d->dy_row, d->D, d->type) && wide(d->dx, d->dx_batch, d->dx_row, d->D, d->type) &&
-                            wide(d->dgate, d->dgate_batch, d->dgate_row, d->D, d->type));
-  if (d->type == 0) launch<FWD, 0>(a, w, blocks, s);
-  else if (d->type == 1) launch<FWD, 1>(a, w, blocks, s);
-  else launch<FWD, 2>(a, w, blocks, s);
+  if (forward) hipLaunchKernelGGL((scan_fwd_kernel<TYPE, WIDE>), dim3(chains * a.units), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((scan_bwd_kernel<TYPE, WIDE>), dim3(chains * a.units), dim3(256), 0, s, a);
   VMM_LAUNCH_CHECK();
   return 0;
+}
+
+int scan(const vmm_gated_scan_desc* d, bool forward, hipStream_t s) {
+  const Layout l = layout(d, !forward);
+  if (l.bytes > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15))) return -1;
+  ScanArgs a = {};
+  a.d = *d;
+  a.tiles = (d->D + CG * V - 1) / (CG * V);
+  a.units = l.units;
+  a.groups = l.groups;
+  if ((u64)l.units * d->B * a.tiles >= (1ull << 31)) return -1;
+  char* w = (char*)d->workspace;
+  a.maps = (float2*)w;
+  a.group_maps = (float2*)(w + l.group_maps);
+  a.anchors = (float*)(w + l.anchors);
+  a.states = forward && d->states ? d->states : (float*)(w + l.states);
+  const auto ok = [&](const void* p, int64_t batch, int64_t row) { return wide(p, batch, row, d->D, d->type); };
+  const bool w4 = ok(d->x, d->x_batch, d->x_row) && ok(d->gate, d->gate_batch, d->gate_row) &&
+                  (forward ? ok(d->y, d->y_batch, d->y_row)
+                           : ok(d->dy, d->dy_batch, d->dy_row) && ok(d->dx, d->dx_batch, d->dx_row) && ok(d->dgate, d->dgate_batch, d->dgate_row));
+  switch (d->type * 2 + (w4 ? 1 : 0)) {
+    case 0: return run<0, false>(a, forward, s);
+    case 1: return run<0, true>(a, forward, s);
+    case 2: return run<1, false>(a, forward, s);
+    case 3: return run<1, true>(a, forward, s);
+    case 4: return run<2, false>(a, forward, s);
+    default: return run<2, true>(a, forward, s);
+  }
 }
 
 // no steps: the state passes through, and so does its gradient
@@ -563,13 +618,12 @@ int pass(const float* from, float* to, long long n, hipStream_t s) {
 
 extern "C" int64_t vmm_gated_scan_states(const vmm_gated_scan_desc* d) {
   if (bad_scan(d)) return -1;
-  return (d->L + STATE_STEP - 1) / STATE_STEP * d->B * d->D;
+  return (d->L + UNIT - 1) / UNIT * d->B * d->D;
 }
 
 extern "C" int64_t vmm_gated_scan_workspace(const vmm_gated_scan_desc* d, int32_t backward) {
   if (bad_scan(d)) return -1;
-  const Layout l = layout(d, backward != 0);
-  return l.chunks > 1 ? 16 + up16(8 * l.maps) + up16(4 * l.states) : 0;
+  return layout(d, backward != 0).bytes;
 }
 
 extern "C" int vmm_gated_scan(const vmm_gated_scan_desc* d, vmm_stream_t stream) {
@@ -578,7 +632,7 @@ extern "C" int vmm_gated_scan(const vmm_gated_scan_desc* d, vmm_stream_t stream)
   if (BD == 0) return 0;
   if (d->L == 0) return pass(d->h0, d->h_last, BD, (hipStream_t)stream);
   if (!d->x || !d->gate || !d->y) return -1;
-  return scan<true>(d, (hipStream_t)stream);
+  return scan(d, true, (hipStream_t)stream);
 }
 
 extern "C" int vmm_gated_scan_bwd(const vmm_gated_scan_desc* d, vmm_stream_t stream) {
@@ -587,5 +641,5 @@ extern "C" int vmm_gated_scan_bwd(const vmm_gated_scan_desc* d, vmm_stream_t str
   if (BD == 0) return 0;
   if (d->L == 0) return pass(d->dh_last, d->dh0, BD, (hipStream_t)stream);
   if (!d->x || !d->gate || !d->states) return -1;
-  return scan<false>(d, (hipStream_t)stream);
+  return scan(d, false, (hipStream_t)stream);
 }
