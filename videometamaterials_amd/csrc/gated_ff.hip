@@ -308,43 +308,92 @@ __global__ __launch_bounds__(256) void ff_layin_kernel(const Layin a) {
   }
 }
 
-// ---- backward, first: dg and du as operands (rounded to the type, or split) and the partial column sums of a run of rows
-template <int TYPE>
+// ---- backward, first: dg and du as operands (rounded to the type, or split) and the column sums of a run of rows.  64 lanes of 4 columns x 4 rows.
+template <int TYPE, bool WIDE>
 __global__ __launch_bounds__(256) void ff_dact_kernel(const vmm_gated_ff_desc d, u16* dg, u16* du, int pitch, int run, float* __restrict__ sums) {
   typedef typename Elem<TYPE>::T T;
-  const int f = blockIdx.x * 256 + threadIdx.x;
-  if (f >= pitch) return;
-  const long long plane = d.M * pitch;
-  float sg = 0.f, su = 0.f;
-  const long long m1 = min((long long)d.M, (long long)(blockIdx.y + 1) * run);
-  for (long long m = (long long)blockIdx.y * run; m < m1; ++m) {
-    float vg = 0.f, vu = 0.f;
-    if (f < d.F) {
-      const float dh = (float)((const T*)d.dh)[m * d.lddh + f];
-      float a, slope;
-      act_both(d.g_pre[m * d.F + f], d.act, a, slope);
-      vg = dh * d.u_pre[m * d.F + f] * slope;
-      vu = dh * a;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  typedef u16 U4 __attribute__((ext_vector_type(4)));
+  __shared__ float part[4][2][256];
+  const int lane = threadIdx.x & 63, row = threadIdx.x >> 6, f = (blockIdx.x * 64 + lane) * 4;
+  const long long plane = d.M * pitch, m1 = min((long long)d.M, (long long)(blockIdx.y + 1) * run);
+  float sg[4] = {}, su[4] = {};
+  if (f < pitch) {
+#pragma unroll 4
+    for (long long m = (long long)blockIdx.y * run + row; m < m1; m += 4) {
+      float g[4], u[4], dh[4];
+      const T* hp = (const T*)d.dh + m * d.lddh + f;
+      const float *gp = d.g_pre + m * d.F + f, *up = d.u_pre + m * d.F + f;
+      if constexpr (WIDE) {
+        T4 hv = {};
+        f32x4 gv = {}, uv = {};
+        if (f < d.F) {
+          hv = *reinterpret_cast<const T4*>(hp);
+          gv = *reinterpret_cast<const f32x4*>(gp);
+          uv = *reinterpret_cast<const f32x4*>(up);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { dh[j] = (float)hv[j]; g[j] = gv[j]; u[j] = uv[j]; }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool in = f + j < d.F;
+          dh[j] = in ? (float)hp[j] : 0.f;
+          g[j] = in ? gp[j] : 0.f;
+          u[j] = in ? up[j] : 0.f;
+        }
+      }
+      u16 og[3][4], ou[3][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float a, slope;
+        act_both(g[j], d.act, a, slope);
+        const float vg = dh[j] * u[j] * slope, vu = dh[j] * a;
+        sg[j] += vg;
+        su[j] += vu;
+        put<TYPE>(&og[0][j], 4, vg);
+        put<TYPE>(&ou[0][j], 4, vu);
+      }
+#pragma unroll
+      for (int p = 0; p < Elem<TYPE>::PLANES; ++p) {
+        *reinterpret_cast<U4*>(dg + p * plane + m * pitch + f) = U4{og[p][0], og[p][1], og[p][2], og[p][3]};
+        *reinterpret_cast<U4*>(du + p * plane + m * pitch + f) = U4{ou[p][0], ou[p][1], ou[p][2], ou[p][3]};
+      }
     }
-    put<TYPE>(dg + m * pitch + f, plane, vg);
-    put<TYPE>(du + m * pitch + f, plane, vu);
-    sg += vg;
-    su += vu;
   }
-  if (sums && f < d.F) {
-    sums[(long long)blockIdx.y * 2 * d.F + f] = sg;
-    sums[(long long)blockIdx.y * 2 * d.F + d.F + f] = su;
+  if (!sums) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    part[row][0][lane * 4 + j] = sg[j];
+    part[row][1][lane * 4 + j] = su[j];
+  }
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < d.F) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      sums[((long long)blockIdx.y * 2 + k) * d.F + c] = (part[0][k][threadIdx.x] + part[1][k][threadIdx.x]) + (part[2][k][threadIdx.x] + part[3][k][threadIdx.x]);
   }
 }
+// 32 columns x 8 lanes that share the runs
 template <int TYPE>
 __global__ __launch_bounds__(256) void ff_dbias_kernel(const vmm_gated_ff_desc d, const float* __restrict__ sums, int runs) {
   typedef typename Elem<TYPE>::T T;
-  const int f = blockIdx.x * 256 + threadIdx.x;
-  if (f >= 2 * d.F) return;
+  __shared__ float part[8][32];
+  const int col = threadIdx.x & 31, share = threadIdx.x >> 5;
+  const long long f = (long long)blockIdx.x * 32 + col;
   float s = 0.f;
-  for (int r = 0; r < runs; ++r) s += sums[(long long)r * 2 * d.F + f];
-  if (f < d.F) { if (d.db_gate) ((T*)d.db_gate)[f] = (T)s; }
-  else if (d.db_up) ((T*)d.db_up)[f - d.F] = (T)s;
+  if (f < 2LL * d.F) {
+#pragma unroll 4
+    for (int r = share; r < runs; r += 8) s += sums[(long long)r * 2 * d.F + f];
+  }
+  part[share][col] = s;
+  __syncthreads();
+  if (share == 0 && f < 2LL * d.F) {
+    for (int k = 1; k < 8; ++k) s += part[k][col];
+    if (f < d.F) { if (d.db_gate) ((T*)d.db_gate)[f] = (T)s; }
+    else if (d.db_up) ((T*)d.db_up)[f - d.F] = (T)s;
+  }
 }
 
 // ---- host side
@@ -359,15 +408,16 @@ bool bad_ff(const vmm_gated_ff_desc* d) {
 }
 
 // The tiles and runs of a product.  Big tiles read LDS 0.75 times per matrix instruction slot where small ones read it as often as it can be read; they
-// are taken where they fill the card.  A product with fewer tiles than CUs is cut along its reduced length, by four steps a run at the least.
+// are taken where they fill the card.  Products whose tiles do not put two workgroups on every
+// CU are cut along their reduced length, by four steps a run at the least.
 struct Shape { bool big; int splits; };
 Shape shape_of(long long rows, long long cols, bool gated, long long units, int products) {
   const auto tiles = [&](long long r) { return ((rows + r - 1) / r) * ((cols * (gated ? 2 : 1) + r - 1) / r) * products; };
   Shape s;
   s.big = tiles(256) >= 192;
-  const long long t = tiles(s.big ? 256 : 128);
+  const long long t = tiles(s.big ? 256 : 128) * (s.big ? 2 : 1);
   long long n = 1;
-  if (t < 256) n = 512 / t;
+  if (t < 512) n = (512 + t / 2) / t;
   if (n > units / 4) n = units / 4;
   if (n > 64) n = 64;
   s.splits = (int)(n < 1 ? 1 : n);
@@ -402,7 +452,9 @@ Layout layout(const vmm_gated_ff_desc* d, bool backward) {
   if (backward) {
     l.dg = take(2LL * l.planes * d->M * l.fp);
     l.du = take(2LL * l.planes * d->M * l.fp);
-    l.run = (int)(d->M <= 64 * 1024 ? 64 : up((d->M + 1023) / 1024, 64));
+    // runs of rows for the activation's backward: four workgroups a CU, 64 rows a run at the most unless the runs became too many
+    const long long columns = (l.fp + 255) / 256, share = up((d->M * columns + 1023) / 1024, 4);
+    l.run = (int)(share < 64 ? share : d->M <= 64 * 1024 ? 64 : up((d->M + 1023) / 1024, 4));
     l.runs = (int)((d->M + l.run - 1) / l.run);
     l.sums = take(8LL * l.runs * d->F);
     const long long px = l.dx.splits > 1 && d->dx ? 4LL * l.dx.splits * d->M * d->K : 0, pw = l.dw.splits > 1 && d->dw_gate ? 8LL * l.dw.splits * d->F * d->K : 0;
@@ -484,11 +536,14 @@ int backward(const vmm_gated_ff_desc* d, hipStream_t s) {
   float* sums = bias ? (float*)(w + l.sums) : nullptr;
   u16 *dg = (u16*)(w + l.dg), *du = (u16*)(w + l.du);
   if (d->M > 0) {
-    hipLaunchKernelGGL(ff_dact_kernel<TYPE>, dim3(cdiv(l.fp, 256), l.runs), dim3(256), 0, s, *d, dg, du, l.fp, l.run, sums);
+    const bool wide = d->F % 4 == 0 && d->lddh % 4 == 0 && ((uintptr_t)d->dh & (4 * esize(d->type) - 1)) == 0 && (((uintptr_t)d->g_pre | (uintptr_t)d->u_pre) & 15) == 0;
+    const dim3 grid(cdiv(l.fp, 256), l.runs);
+    if (wide) hipLaunchKernelGGL((ff_dact_kernel<TYPE, true>), grid, dim3(256), 0, s, *d, dg, du, l.fp, l.run, sums);
+    else hipLaunchKernelGGL((ff_dact_kernel<TYPE, false>), grid, dim3(256), 0, s, *d, dg, du, l.fp, l.run, sums);
     VMM_LAUNCH_CHECK();
   }
   if (bias) {
-    hipLaunchKernelGGL(ff_dbias_kernel<TYPE>, dim3(cdiv(2LL * d->F, 256)), dim3(256), 0, s, *d, (const float*)sums, l.runs);
+    hipLaunchKernelGGL(ff_dbias_kernel<TYPE>, dim3(cdiv(2LL * d->F, 32)), dim3(256), 0, s, *d, (const float*)sums, l.runs);
     VMM_LAUNCH_CHECK();
   }
   Operands o;

@@ -6,10 +6,10 @@ over the gradients -- or ``DataParallelTrainer(max_grad_norm=...)``.
 """
 from __future__ import annotations
 
-import ctypes as C
 from operator import attrgetter
 from typing import Iterable, List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from . import _native as N
@@ -21,6 +21,11 @@ _dtype = attrgetter("dtype")
 def on_device(index: int):
     """The device of a call's tensors made current for its launches, where another one is."""
     return torch.cuda.device(index if index != torch.cuda.current_device() else -1)
+
+
+def stream_of(index: int) -> int:
+    """Handle of the current stream of a device."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _same_device(tensors: Sequence[torch.Tensor], what: str) -> int:
@@ -50,22 +55,30 @@ def _as_list(tensors, what: str) -> List[torch.Tensor]:
     return tensors
 
 
-def _grad_jobs(tensors: Sequence[torch.Tensor]):
-    jobs = (N.GradJob * len(tensors))()
-    for job, p, n, t in zip(jobs, map(torch.Tensor.data_ptr, tensors), map(torch.Tensor.numel, tensors), map(_dtype, tensors)):
-        job.g, job.n, job.type = p, n, TYPES[t]
+# the job structs of include/vmm_sequence.h as rows of an array: hundreds of tensors are filled in column by column
+GRAD_JOB = np.dtype([("g", np.uint64), ("n", np.int64), ("type", np.int32), ("reserved", np.int32)])
+ADAM_JOB = np.dtype([("p", np.uint64), ("g", np.uint64), ("m", np.uint64), ("v", np.uint64), ("n", np.int64), ("type", np.int32), ("reserved", np.int32)])
+
+
+def _grad_jobs(tensors: Sequence[torch.Tensor]) -> np.ndarray:
+    jobs = np.zeros(len(tensors), GRAD_JOB)
+    jobs["g"] = list(map(torch.Tensor.data_ptr, tensors))
+    jobs["n"] = list(map(torch.Tensor.numel, tensors))
+    kinds = list(map(_dtype, tensors))
+    first = kinds[0]
+    jobs["type"] = TYPES[first] if kinds.count(first) == len(kinds) else [TYPES[k] for k in kinds]
     return jobs
 
 
-def _norm(jobs, n: int, max_norm: float, device: int, scale: float = 1.0) -> torch.Tensor:
+def _norm(jobs, n: int, max_norm: float, index: int, scale: float = 1.0) -> torch.Tensor:
     """(norm, factor) on the device; max_norm <= 0: the factor is one."""
     lib = N.lib()
-    size = lib.vmm_grad_norm_workspace(jobs, n)
+    size = lib.vmm_grad_norm_workspace(jobs.ctypes.data, n)
     if size < 0:
         raise ValueError("gradient norm: a tensor that is not aligned to its type")
-    work = torch.empty(size // 8 + 1, dtype=torch.float64, device=device)  # (the last one holds the two results)
+    work = torch.empty(size // 8 + 1, dtype=torch.float64, device=index)  # (the last one holds the two results)
     out = work[size // 8:].view(torch.float32)
-    N.check(lib.vmm_grad_norm(jobs, n, scale, max_norm, None, work.data_ptr(), out.data_ptr(), C.c_void_p(torch.cuda.current_stream().cuda_stream)),
+    N.check(lib.vmm_grad_norm(jobs.ctypes.data, n, scale, max_norm, None, work.data_ptr(), out.data_ptr(), stream_of(index)),
             "vmm_grad_norm")
     return out
 
@@ -97,7 +110,7 @@ def clip_grad_norm_(grads: Iterable[torch.Tensor], max_norm: float) -> torch.Ten
     with on_device(index):
         jobs = _grad_jobs(grads)
         out = _norm(jobs, len(grads), max_norm, index)
-        code = N.lib().vmm_grad_clip(jobs, len(grads), out.data_ptr(), C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        code = N.lib().vmm_grad_clip(jobs.ctypes.data, len(grads), out.data_ptr(), stream_of(index))
         if code == -2:
             raise ValueError("clip_grad_norm_: tensors overlap in memory")
         N.check(code, "vmm_grad_clip")
@@ -131,9 +144,10 @@ class ClippedAdam:
             if len(ts) != len(self.params) or list(map(torch.Tensor.numel, ts)) != self._sizes:
                 raise ValueError(f"ClippedAdam: {name} do not fit the parameters")
         self._device = self._check_own()
-        self._jobs = (N.ClipAdamJob * len(self.params))()
-        for job, m, v, n in zip(self._jobs, self.exp_avgs, self.exp_avg_sqs, self._sizes):
-            job.m, job.v, job.n = m.data_ptr(), v.data_ptr(), n
+        self._jobs = np.zeros(len(self.params), ADAM_JOB)
+        self._jobs["m"] = list(map(torch.Tensor.data_ptr, self.exp_avgs))
+        self._jobs["v"] = list(map(torch.Tensor.data_ptr, self.exp_avg_sqs))
+        self._jobs["n"] = self._sizes
         self._at: List[int] = []
 
     def _check_own(self) -> int:
@@ -165,19 +179,15 @@ class ClippedAdam:
         if at != self._at:  # first step, or parameters were re-homed
             if self._check_own() != self._device or list(map(torch.Tensor.numel, self.params)) != self._sizes:
                 raise ValueError("ClippedAdam.step: parameters were moved to another device or resized")
-            for job, p in zip(self._jobs, at):
-                job.p = p
+            self._jobs["p"] = at
             self._at = at
         with on_device(self._device):
-            jobs = self._jobs
-            if len(here) < len(self.params):
-                jobs = (N.ClipAdamJob * len(here))(*[self._jobs[i] for i in here])
+            jobs = self._jobs if len(here) == len(self.params) else self._jobs[here]
             norm_jobs = _grad_jobs(grads)
-            for job, g in zip(jobs, norm_jobs):
-                job.g, job.type = g.g, g.type
+            jobs["g"], jobs["type"] = norm_jobs["g"], norm_jobs["type"]
             out = _norm(norm_jobs, len(grads), self.max_norm or 0.0, self._device)
-            code = N.lib().vmm_adam_step_clipped(jobs, len(here), self.lr, self.betas[0], self.betas[1], self.eps, self.steps_taken + 1, 1.0, out.data_ptr(),
-                                                 None, C.c_void_p(torch.cuda.current_stream().cuda_stream))
+            code = N.lib().vmm_adam_step_clipped(jobs.ctypes.data, len(here), self.lr, self.betas[0], self.betas[1], self.eps, self.steps_taken + 1, 1.0, out.data_ptr(),
+                                                 None, stream_of(self._device))
             if code == -2:
                 raise ValueError("ClippedAdam.step: parameters, moments or gradients overlap in memory")
             N.check(code, "vmm_adam_step_clipped")

@@ -10,13 +10,9 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native as N
-from .optim import TYPES, on_device
+from .optim import TYPES, on_device, stream_of
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
-
-
-def _stream() -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
 def _need_gpu(t: torch.Tensor, what: str) -> None:
@@ -69,7 +65,7 @@ def _scan_forward(x, gate, h0, lengths, keep: bool):
             states = torch.empty(max(lib.vmm_gated_scan_states(C.byref(d)), 0), dtype=torch.float32, device=x.device)
             d.states = states.data_ptr()
         work = _scan_workspace(lib, d, 0, x.device)  # noqa: F841 (alive until the launch is enqueued)
-        N.check(lib.vmm_gated_scan(C.byref(d), _stream()), "vmm_gated_scan")
+        N.check(lib.vmm_gated_scan(C.byref(d), stream_of(x.get_device())), "vmm_gated_scan")
     return y, h_last, states
 
 
@@ -96,7 +92,7 @@ class _GatedScan(torch.autograd.Function):
             dh0 = torch.empty((B, D), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
             d = _scan_desc(x, gate, None, lengths, states=states, dy=dy, dx=dx, dgate=dgate, dh_last=dh_last, dh0=dh0)
             work = _scan_workspace(lib, d, 1, x.device)  # noqa: F841
-            N.check(lib.vmm_gated_scan_bwd(C.byref(d), _stream()), "vmm_gated_scan_bwd")
+            N.check(lib.vmm_gated_scan_bwd(C.byref(d), stream_of(x.get_device())), "vmm_gated_scan_bwd")
         return dx, dgate, dh0, None
 
 
@@ -164,7 +160,7 @@ def _ff_forward(x, wg, wu, bg, bu, act: int, keep: bool):
         pre = torch.empty((2, M, F), dtype=torch.float32, device=x.device) if keep else (None, None)
         d = _ff_desc(x, wg, wu, bg, bu, act, h=h, g_pre=pre[0], u_pre=pre[1])
         work = _ff_workspace(lib, d, 0, x.device)  # noqa: F841 (alive until the launch is enqueued)
-        N.check(lib.vmm_gated_ff(C.byref(d), _stream()), "vmm_gated_ff")
+        N.check(lib.vmm_gated_ff(C.byref(d), stream_of(x.get_device())), "vmm_gated_ff")
     return h, pre if keep else None
 
 
@@ -190,7 +186,7 @@ class _GatedFF(torch.autograd.Function):
             dbg, dbu = torch.empty((2, wg.shape[0]), dtype=x.dtype, device=x.device) if biases else (None, None)
             d = _ff_desc(x, wg, wu, None, None, ctx.act, g_pre=pre[0], u_pre=pre[1], dh=dh, dx=dx, dwg=dwg, dwu=dwu, dbg=dbg, dbu=dbu)
             work = _ff_workspace(lib, d, 1, x.device)  # noqa: F841
-            N.check(lib.vmm_gated_ff_bwd(C.byref(d), _stream()), "vmm_gated_ff_bwd")
+            N.check(lib.vmm_gated_ff_bwd(C.byref(d), stream_of(x.get_device())), "vmm_gated_ff_bwd")
         return dx, *(t if n else None for t, n in zip((dwg, dwu, dbg, dbu), need[1:5])), None
 
 
