@@ -13,8 +13,8 @@
 //
 // A tile step is 64 reduced indexes.  It goes from memory to LDS directly (buffer loads with an LDS destination: no registers, and what lies
 // outside the operand arrives as zero), into the one of two buffers that the matrix instructions do not read.  Such a load fills 1 KiB of LDS in lane order,
-// so the banks are spread by which 16 bytes each lane FETCHES: row-contiguous operands swap 16-byte pieces by the row's lower three bits (read back with
-// 16-byte reads), column-contiguous ones by the lower two bits of k (read back with the transposing 8-byte reads).
+// so the banks are spread by which 16 bytes each lane FETCHES: row-contiguous operands swap 16-byte pieces by bits 1..3 of the row (16 lanes read 16
+// rows at once, and rows two apart start at the same bank), column-contiguous ones by the lower two bits of k (read back with the transposing 8-byte reads).
 #include "vmm_common.h"
 #include "../../include/vmm_kernels.h"
 
@@ -82,8 +82,9 @@ __device__ __forceinline__ int acc_row(int r) { return (r >> 2) * 8 + ((threadId
 template <bool COL, int R, int WAVES>
 struct Loader {
   static constexpr int LOADS = R / 8 / WAVES;
+  static_assert(LOADS % 2 == 0, "a wave's loads start at an even row of pieces");
   unsigned off[LOADS];  // byte offset of this lane's 16 bytes from the tile's first value
-  int kc;               // row-contiguous: first k of the lane's piece
+  int kc;               // row-contiguous: first k of the lane's piece in even loads; in odd ones it is 32 away
   long long ld, left;
   // r0: first row of the tile of the `rows`; FOLD: rows 32..63 of every 64 are rows 0..31 of the same 32 in a second matrix
   template <bool FOLD>
@@ -91,7 +92,7 @@ struct Loader {
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     ld = ld_;
     left = rows - r0;
-    kc = ((lane & 7) ^ (lane >> 3)) * 8;
+    kc = ((lane & 7) ^ (lane >> 4)) * 8;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int piece = (wave * LOADS + i) * 64 + lane;  // of 16 bytes, in LDS order
@@ -101,7 +102,7 @@ struct Loader {
       } else {
         int r = piece / 8;
         if constexpr (FOLD) r = (r >> 6) * 32 + (r & 31);
-        off[i] = r < left ? (unsigned)(r * ld * 2 + kc * 2) : 0xfffffff0u;
+        off[i] = r < left ? (unsigned)(r * ld * 2 + (kc ^ (i & 1) * 32) * 2) : 0xfffffff0u;
       }
     }
   }
@@ -113,7 +114,7 @@ struct Loader {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(base), 0, (int)size, 0x00027000);
     const int wave = uniform(threadIdx.x >> 6);
     unsigned o = off[i];
-    if (!COL && kc >= rest) o = 0xfffffff0u;
+    if (!COL && (kc ^ (i & 1) * 32) >= rest) o = 0xfffffff0u;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(tile + (wave * LOADS + i) * 512), 16, o, 0, 0, 0);
   }
 };
@@ -131,7 +132,7 @@ __device__ __forceinline__ uint4 fragment(const u16* tile, int r0, int ks) {
     const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
     return make_uint4(l.x, l.y, h.x, h.y);
   } else {
-    const int r = r0 + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ (r & 7);
+    const int r = r0 + (lane & 31), c = (ks * 2 + (lane >> 5)) ^ ((r >> 1) & 7);
     return *reinterpret_cast<const uint4*>(tile + r * BK + c * 8);
   }
 }
