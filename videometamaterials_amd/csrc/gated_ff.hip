@@ -46,6 +46,7 @@ struct Gemm {
   int parts, splits;                // the reduced length (of all parts) is cut into `splits` runs
   long long tiles_m, tiles_n;
   void* out[2]; long long ldo;      // one run
+  bool pairs;                       // rows of `out` and their length are even: results of 16 bits can leave in pairs
   float* partial;                   // several: [product][run][rows][cols], forward [run][2][rows][cols]
   // forward
   const void* b_gate; const void* b_up; float* g_pre; float* u_pre; int act;
@@ -60,23 +61,98 @@ __device__ __forceinline__ const u16* uniform(const u16* p) {
   return (const u16*)((unsigned long long)hi << 32 | lo);
 }
 
-__device__ __forceinline__ float act_of(float g, int act) {
-  return act == 0 ? g / (1.0f + expf(-g)) : 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
-}
-__device__ __forceinline__ void act_both(float g, int act, float& a, float& slope) {
-  if (act == 0) {
-    const float p = 1.0f / (1.0f + expf(-g));
-    a = g * p;
-    slope = p * (1.0f + g * (1.0f - p));
+// e^-m, m >= 0.  In 16 bits the hardware's 2^p of the rounded p = -m log2(e) does; fp32 corrects for what the rounding has lost, up to m 2^-25 of the result.
+template <int TYPE>
+__device__ __forceinline__ float exp_minus(float m) {
+  if constexpr (TYPE == 0) {
+    m = m > 104.f ? 104.f : m;  // (zero from there on; an infinite one would leave inf - inf below)
+    const float p = m * -1.44269502162933349609375f;
+    float t = fmaf(m, -1.44269502162933349609375f, -p);
+    t = fmaf(m, -1.925963033500011e-08f, t);
+    const float e = __builtin_amdgcn_exp2f(p);
+    return fmaf(e, t * 0.6931471805599453f, e);
   } else {
-    const float p = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-    a = g * p;
-    slope = p + g * expf(-0.5f * g * g) * 0.39894228040143268f;
+    return __builtin_amdgcn_exp2f(m * -1.44269502162933349609375f);
   }
+}
+// The activation's factor P (a = g P) and its derivative P + g P'.
+//   silu: P = sigmoid(g) from e^-|g|, P' = P (1 - P)
+//   gelu: P = Phi(g), the normal distribution: Phi(-|g|) = e^(-g^2/2) erfcx(|g| / sqrt 2) / 2, whose last two factors are a polynomial in
+//         t = 1 / (1 + |g| / sqrt 8), fitted for the least relative error over |g| <= 13.4 (4.2e-8; 3.2e-7 as evaluated); P' = e^(-g^2/2) / sqrt(2 pi)
+// (erff and the exact division took half of the epilogue: 512 x 256 x 128 values, 13 us a tile)
+template <int TYPE, int ACT, bool SLOPE>
+__device__ __forceinline__ float act_parts(float g, float& slope) {
+  const float m = fabsf(g);
+  if constexpr (ACT == 0) {
+    const float e = exp_minus<TYPE>(m), r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r, p = g < 0.f ? er : r;
+    if constexpr (SLOPE) slope = p * fmaf(g, g < 0.f ? r : er, 1.0f);
+    return g * p;
+  } else {
+    const float t = __builtin_amdgcn_rcpf(fmaf(m, 0.35355339059327376f, 1.0f)), e = exp_minus<TYPE>(0.5f * g * g);
+    float q = -0.029445331543684006f;
+    q = fmaf(q, t, 0.14185069501399994f);
+    q = fmaf(q, t, -0.2426912486553192f);
+    q = fmaf(q, t, 0.1379883736371994f);
+    q = fmaf(q, t, -0.012588338926434517f);
+    q = fmaf(q, t, 0.10103470087051392f);
+    q = fmaf(q, t, 0.12163055688142776f);
+    q = fmaf(q, t, 0.1411767303943634f);
+    q = fmaf(q, t, 0.14104384183883667f);
+    q *= t * e;
+    const float p = g < 0.f ? q : 1.0f - q;
+    if constexpr (SLOPE) slope = fmaf(g * e, 0.3989422804014327f, p);
+    return g * p;
+  }
+}
+template <int TYPE, int ACT>
+__device__ __forceinline__ float act_of(float g) {
+  float slope;
+  return act_parts<TYPE, ACT, false>(g, slope);
 }
 
 // row of accumulator register r of a 32 x 32 tile (its column is the lane's lower five bits)
 __device__ __forceinline__ int acc_row(int r) { return (r >> 2) * 8 + ((threadIdx.x & 63) >> 5) * 4 + (r & 3); }
+
+// A 32 x 32 tile of results to rows of T from row m, column n on (the same for all lanes: the address of a row is, and the lane's part is 32 bits).
+// One value after the other (the empty asm): computed side by side they would need more registers than there are and the steps' loop would spill.
+// PAIRS: even rows and columns, so that lanes exchange a value for each two and 16-bit results leave two at a time.
+template <typename T, typename F>
+__device__ __forceinline__ void put_tile(T* out, long long ldo, long long rows, long long cols, long long m, long long n, bool pairs, F value) {
+  const int lane = threadIdx.x & 63, col = lane & 31, row0 = (lane >> 5) * 4;
+  const int rows_left = (int)min(rows - m, 32LL) - row0, cols_left = (int)min(cols - n, 32LL);
+  char* base = (char*)(out + m * ldo + n);
+  const long long pitch = ldo * (long long)sizeof(T);
+  if constexpr (sizeof(T) == 2) {
+    if (pairs) {
+      typedef T T2 __attribute__((ext_vector_type(2)));
+      typedef float f32x2_t __attribute__((ext_vector_type(2)));
+      const int odd = col & 1;
+      const unsigned off = (unsigned)((row0 + odd) * (int)pitch) + (col & ~1) * 2;
+      if (col < cols_left) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          float v0 = value(r), v1 = value(r + 1);
+          asm volatile("" : "+v"(v0), "+v"(v1)::"memory");
+          const float other = lane_xor(odd ? v0 : v1, 0);
+          const f32x2_t v = {odd ? other : v0, odd ? v1 : other};
+          const int at = (r >> 2) * 8 + (r & 3);
+          if (at + odd < rows_left) *reinterpret_cast<T2*>(base + at * pitch + off) = __builtin_convertvector(v, T2);
+        }
+      }
+      return;
+    }
+  }
+  const unsigned off = (unsigned)(row0 * (int)pitch) + col * (unsigned)sizeof(T);
+  if (col < cols_left) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int at = (r >> 2) * 8 + (r & 3);
+      float v = value(r);
+      asm volatile("" : "+v"(v)::"memory");
+      if (at < rows_left) *reinterpret_cast<T*>(base + at * pitch + off) = (T)v;
+    }
+  }
+}
 
 // ---- one operand's tile of R rows.  Every wave issues R / 8 / WAVES loads of 1 KiB.
 template <bool COL, int R, int WAVES>
@@ -149,7 +225,7 @@ __global__ __launch_bounds__(BIG ? 512 : 256, BIG ? 2 : 2) void ff_gemm_kernel(c
   const unsigned tiles = (unsigned)(q.tiles_m * q.tiles_n), per = (tiles + 7) / 8, t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (t >= tiles) return;
   const unsigned in_all = 8 * (unsigned)q.tiles_n, band = t / in_all, bm = min(8u, (unsigned)q.tiles_m - band * 8), in_band = t - band * in_all;
-  const long long m0 = (long long)uniform(band * 8 + in_band % bm) * R, n0 = (long long)uniform(in_band / bm) * (GATED ? R / 2 : R);
+  long long m0 = (long long)uniform(band * 8 + in_band % bm) * R, n0 = (long long)uniform(in_band / bm) * (GATED ? R / 2 : R);
   const int run = uniform(blockIdx.y % q.splits), prod = uniform(blockIdx.y / q.splits);
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = BIG ? (wave & 1) * 128 : (wave & 1) * 64, wn = (wave >> 1) * 64;
@@ -194,61 +270,58 @@ __global__ __launch_bounds__(BIG ? 512 : 256, BIG ? 2 : 2) void ff_gemm_kernel(c
         for (int j = 0; j < 2; ++j) acc[i][j] = mfma<HALF>(a[i], b[j], acc[i][j]);
     }
   };
-  if (u0 < u1) fetch(a0, b0);
-  for (int u = u0; u < u1; u += 2) {
-    __syncthreads();  // this wave's loads have landed, and every wave's after the barrier; nobody reads the other buffer any more
-    if (u + 1 < u1) fetch(a1, b1);
+  // At each barrier this wave's loads of the step have landed, and every wave's behind it; nobody reads the other buffer any more.
+  int u = u0;
+  if (u < u1) fetch(a0, b0);
+  for (; u + 1 < u1; u += 2) {
+    __syncthreads();
+    fetch(a1, b1);
     compute(a0, b0);
-    if (u + 1 >= u1) break;
     __syncthreads();
     if (u + 2 < u1) fetch(a0, b0);
     compute(a1, b1);
   }
+  if (u < u1) {
+    __syncthreads();
+    compute(a0, b0);
+  }
 
+  // (what follows starts from values that exist only here: worked out ahead of the steps, its addresses would take the registers of the operands)
+  int here = 0;
+  asm volatile("" : "+s"(here));
+  m0 += here;
+  n0 += here;
   if constexpr (GATED) {
-    const long long f = n0 + wn / 2 + (lane & 31);
-    if (f >= q.cols) return;
+    const long long fn = n0 + wn / 2, f = fn + (lane & 31);
     if (q.splits > 1) {
       float* pg = q.partial + (long long)run * 2 * q.rows * q.cols;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const long long m = m0 + wm + i * 32 + acc_row(r);
-          if (m < q.rows) {
-            pg[m * q.cols + f] = acc[i][0][r];
-            pg[(q.rows + m) * q.cols + f] = acc[i][1][r];
-          }
-        }
+        for (int j = 0; j < 2; ++j)
+          put_tile(pg + j * q.rows * q.cols, q.cols, q.rows, q.cols, m0 + wm + i * 32, fn, false, [&](int r) { return acc[i][j][r]; });
       return;
     }
-    const float bg = q.b_gate ? (float)((const T*)q.b_gate)[f] : 0.f, bu = q.b_up ? (float)((const T*)q.b_up)[f] : 0.f;
+    const float bg = q.b_gate && f < q.cols ? (float)((const T*)q.b_gate)[f] : 0.f, bu = q.b_up && f < q.cols ? (float)((const T*)q.b_up)[f] : 0.f;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const long long m = m0 + wm + i * 32 + acc_row(r);
-        if (m >= q.rows) continue;
-        const float g = acc[i][0][r] + bg, v = acc[i][1][r] + bu;
-        ((T*)q.out[0])[m * q.ldo + f] = (T)(act_of(g, q.act) * v);
-        if (q.g_pre) {
-          q.g_pre[m * q.cols + f] = g;
-          q.u_pre[m * q.cols + f] = v;
-        }
+    for (int i = 0; i < MT; ++i) {
+      if (q.g_pre) {
+        put_tile(q.g_pre, q.cols, q.rows, q.cols, m0 + wm + i * 32, fn, false, [&](int r) { return acc[i][0][r] + bg; });
+        put_tile(q.u_pre, q.cols, q.rows, q.cols, m0 + wm + i * 32, fn, false, [&](int r) { return acc[i][1][r] + bu; });
       }
+      T* h = (T*)q.out[0];
+      if (q.act == 0) put_tile(h, q.ldo, q.rows, q.cols, m0 + wm + i * 32, fn, q.pairs, [&](int r) { return act_of<TYPE, 0>(acc[i][0][r] + bg) * (acc[i][1][r] + bu); });
+      else put_tile(h, q.ldo, q.rows, q.cols, m0 + wm + i * 32, fn, q.pairs, [&](int r) { return act_of<TYPE, 1>(acc[i][0][r] + bg) * (acc[i][1][r] + bu); });
+    }
   } else {
     float* part_out = q.partial + (long long)blockIdx.y * q.rows * q.cols;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const long long m = m0 + wm + i * 32 + acc_row(r), n = n0 + wn + j * 32 + (lane & 31);
-          if (m >= q.rows || n >= q.cols) continue;
-          if (q.splits > 1) part_out[m * q.cols + n] = acc[i][j][r];
-          else ((T*)q.out[prod])[m * q.ldo + n] = (T)acc[i][j][r];
-        }
+      for (int j = 0; j < 2; ++j) {
+        if (q.splits > 1) put_tile(part_out, q.cols, q.rows, q.cols, m0 + wm + i * 32, n0 + wn + j * 32, false, [&](int r) { return acc[i][j][r]; });
+        else put_tile((T*)q.out[prod], q.ldo, q.rows, q.cols, m0 + wm + i * 32, n0 + wn + j * 32, q.pairs, [&](int r) { return acc[i][j][r]; });
+      }
   }
 }
 
@@ -276,7 +349,7 @@ __global__ __launch_bounds__(256) void ff_join_gated_kernel(const Gemm q) {
   }
   g += q.b_gate ? (float)((const T*)q.b_gate)[f] : 0.f;
   u += q.b_up ? (float)((const T*)q.b_up)[f] : 0.f;
-  ((T*)q.out[0])[m * q.ldo + f] = (T)(act_of(g, q.act) * u);
+  ((T*)q.out[0])[m * q.ldo + f] = (T)((q.act == 0 ? act_of<TYPE, 0>(g) : act_of<TYPE, 1>(g)) * u);
   if (q.g_pre) { q.g_pre[i] = g; q.u_pre[i] = u; }
 }
 
@@ -348,7 +421,8 @@ __global__ __launch_bounds__(256) void ff_dact_kernel(const vmm_gated_ff_desc d,
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float a, slope;
-        act_both(g[j], d.act, a, slope);
+        if (d.act == 0) a = act_parts<TYPE, 0, true>(g[j], slope);
+        else a = act_parts<TYPE, 1, true>(g[j], slope);
         const float vg = dh[j] * u[j] * slope, vu = dh[j] * a;
         sg[j] += vg;
         su[j] += vu;
@@ -402,10 +476,11 @@ __global__ __launch_bounds__(256) void ff_dbias_kernel(const vmm_gated_ff_desc d
 inline int esize(int type) { return type == 0 ? 4 : 2; }
 inline long long up(long long n, long long to) { return (n + to - 1) / to * to; }
 
+bool bad_ld(int64_t ld) { return ld < 0 || ld >= (1 << 22); }
 bool bad_ff(const vmm_gated_ff_desc* d) {
   // (K, F < 2^22: a tile of 256 rows is addressed with 32-bit byte offsets)
   return !d || d->M < 0 || d->K < 1 || d->F < 1 || d->K >= (1 << 22) || d->F >= (1 << 22) || d->M >= (1LL << 31) || d->type < 0 || d->type > 2 ||
-         d->act < 0 || d->act > 1 || d->ldx < 0 || d->ldx >= (1 << 22);
+         d->act < 0 || d->act > 1 || bad_ld(d->ldx) || bad_ld(d->ldh) || bad_ld(d->lddx);
 }
 
 // The tiles and runs of a product.  Big tiles read LDS 0.75 times per matrix instruction slot where small ones read it as often as it can be read; they
@@ -473,6 +548,7 @@ int product(Gemm& q, const Shape& sh, int products, hipStream_t s) {
   q.splits = sh.splits;
   q.tiles_m = (q.rows + r - 1) / r;
   q.tiles_n = (q.cols * (GATED ? 2 : 1) + r - 1) / r;
+  q.pairs = q.cols % 2 == 0 && q.ldo % 2 == 0 && (((uintptr_t)q.out[0] | (uintptr_t)q.out[1]) & 3) == 0;
   const long long blocks = (q.tiles_m * q.tiles_n + 7) / 8 * 8;
   if (blocks >= (1LL << 30) || (q.red + BK - 1) / BK * q.parts >= (1LL << 30)) return -1;
   const dim3 grid((unsigned)blocks, products * q.splits);
