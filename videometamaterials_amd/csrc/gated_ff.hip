@@ -15,6 +15,7 @@
 // outside the operand arrives as zero), into the one of two buffers that the matrix instructions do not read.  Such a load fills 1 KiB of LDS in lane order,
 // so the banks are spread by which 16 bytes each lane FETCHES: row-contiguous operands swap 16-byte pieces by bits 1..3 of the row (16 lanes read 16
 // rows at once, and rows two apart start at the same bank), column-contiguous ones by the lower two bits of k (read back with the transposing 8-byte reads).
+#include <algorithm>
 #include "vmm_common.h"
 #include "../../include/vmm_kernels.h"
 
@@ -476,19 +477,25 @@ __global__ __launch_bounds__(256) void ff_dbias_kernel(const vmm_gated_ff_desc d
 inline int esize(int type) { return type == 0 ? 4 : 2; }
 inline long long up(long long n, long long to) { return (n + to - 1) / to * to; }
 
+inline long long cdiv64(long long a, long long b) { return (a + b - 1) / b; }
 bool bad_ld(int64_t ld) { return ld < 0 || ld >= (1 << 22); }
 bool bad_ff(const vmm_gated_ff_desc* d) {
   // (K, F < 2^22: a tile of 256 rows is addressed with 32-bit byte offsets)
-  return !d || d->M < 0 || d->K < 1 || d->F < 1 || d->K >= (1 << 22) || d->F >= (1 << 22) || d->M >= (1LL << 31) || d->type < 0 || d->type > 2 ||
-         d->act < 0 || d->act > 1 || bad_ld(d->ldx) || bad_ld(d->ldh) || bad_ld(d->lddx);
+  if (!d || d->M < 0 || d->K < 1 || d->F < 1 || d->K >= (1 << 22) || d->F >= (1 << 22) || d->M >= (1LL << 31) || d->type < 0 || d->type > 2 || d->act < 0 ||
+      d->act > 1 || bad_ld(d->ldx) || bad_ld(d->ldh) || bad_ld(d->lddx))
+    return true;
+  const auto too_many = [](long long rows, long long cols) { return cdiv64(rows, 256) * cdiv64(cols, 256) >= (1LL << 23) - 8; };  // a launch has less than 2^32 threads
+  return too_many(d->M, 2LL * d->F) || too_many(d->M, d->K) || too_many(d->F, d->K);
 }
 
 // The tiles and runs of a product.  Big tiles read LDS 0.75 times per matrix instruction slot where small ones read it as often as it can be read; they
-// are taken where they fill the card.  Products whose tiles do not put two workgroups on every
-// CU are cut along their reduced length, by four steps a run at the least.
+// are taken where they fill the card (M x K x F of 8192 x 2048 x 8192, bf16, keeping the products: 590 us, small 759; the weight gradients of 1024 x 1024 x
+// 4096, 128 big tiles: 61 us, small 33).  Products whose tiles do not put two workgroups on every CU are cut along their reduced length, by four steps a
+// run at the least (4 x 1024 x 4096 forward: 10.5 us, whole 16.7; dx of 3996 x 1000 x 4096: 136 with the activation's 46, whole 173; a sum that is
+// short for its size loses the time of the join: the weight gradients of 2048 x 1024 x 2048 46, whole 41).
 struct Shape { bool big; int splits; };
 Shape shape_of(long long rows, long long cols, bool gated, long long units, int products) {
-  const auto tiles = [&](long long r) { return ((rows + r - 1) / r) * ((cols * (gated ? 2 : 1) + r - 1) / r) * products; };
+  const auto tiles = [&](long long r) { return std::max(cdiv64(rows, r) * cdiv64(cols * (gated ? 2 : 1), r) * products, 1LL); };  // (no rows: nothing is launched)
   Shape s;
   s.big = tiles(256) >= 192;
   const long long t = tiles(s.big ? 256 : 128) * (s.big ? 2 : 1);
@@ -529,7 +536,7 @@ Layout layout(const vmm_gated_ff_desc* d, bool backward) {
     l.dg = take(2LL * l.planes * d->M * l.fp);
     l.du = take(2LL * l.planes * d->M * l.fp);
     // runs of rows for the activation's backward: four workgroups a CU, 64 rows a run at the most unless the runs became too many
-    const long long columns = (l.fp + 255) / 256, share = up((d->M * columns + 1023) / 1024, 4);
+    const long long columns = (l.fp + 255) / 256, share = up(std::max(cdiv64(d->M * columns, 1024), 1LL), 4);
     l.run = (int)(share < 64 ? share : d->M <= 64 * 1024 ? 64 : up((d->M + 1023) / 1024, 4));
     l.runs = (int)((d->M + l.run - 1) / l.run);
     l.sums = take(8LL * l.runs * d->F);
@@ -550,14 +557,13 @@ int product(Gemm& q, const Shape& sh, int products, hipStream_t s) {
   q.tiles_n = (q.cols * (GATED ? 2 : 1) + r - 1) / r;
   q.pairs = q.cols % 2 == 0 && q.ldo % 2 == 0 && (((uintptr_t)q.out[0] | (uintptr_t)q.out[1]) & 3) == 0;
   const long long blocks = (q.tiles_m * q.tiles_n + 7) / 8 * 8;
-  if (blocks >= (1LL << 30) || (q.red + BK - 1) / BK * q.parts >= (1LL << 30)) return -1;
+  if (cdiv64(q.red, BK) * q.parts >= (1LL << 30)) return -1;
   const dim3 grid((unsigned)blocks, products * q.splits);
   if (sh.big) hipLaunchKernelGGL((ff_gemm_kernel<TYPE, ACOL, BCOL, GATED, true>), grid, dim3(512), 0, s, q);
   else hipLaunchKernelGGL((ff_gemm_kernel<TYPE, ACOL, BCOL, GATED, false>), grid, dim3(256), 0, s, q);
   VMM_LAUNCH_CHECK();
   if (q.splits > 1) {
-    const long long n = (q.rows * q.cols + 255) / 256;
-    if (n >= (1LL << 31)) return -1;
+    const long long n = cdiv64(q.rows * q.cols, 256);  // (less than 512 tiles of 128 x 128, or nothing would be split)
     if constexpr (GATED) hipLaunchKernelGGL(ff_join_gated_kernel<TYPE>, dim3((unsigned)n), dim3(256), 0, s, q);
     else hipLaunchKernelGGL(ff_join_kernel<TYPE>, dim3((unsigned)n, products), dim3(256), 0, s, q);
     VMM_LAUNCH_CHECK();
@@ -580,7 +586,7 @@ int operands(const vmm_gated_ff_desc* d, const Layout& l, Operands& o, hipStream
   o = {(const u16*)(w + l.x), (const u16*)(w + l.wg), (const u16*)(w + l.wu), l.kp, l.kp, d->M * l.kp, (long long)d->F * l.kp};
   const Layin a = {{d->x, d->w_gate, d->w_up}, {(u16*)(w + l.x), (u16*)(w + l.wg), (u16*)(w + l.wu)}, {d->M, d->F, d->F}, {d->ldx, d->K, d->K}, d->K, l.kp};
   const long long most = (d->M > d->F ? d->M : d->F) * (long long)l.kp;
-  hipLaunchKernelGGL(ff_layin_kernel<TYPE>, dim3((unsigned)min(cdiv(most, 256), 4096), 3), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(ff_layin_kernel<TYPE>, dim3((unsigned)std::min(cdiv64(most, 256), 4096LL), 3), dim3(256), 0, s, a);
   VMM_LAUNCH_CHECK();
   return 0;
 }
@@ -623,6 +629,7 @@ int backward(const vmm_gated_ff_desc* d, hipStream_t s) {
     hipLaunchKernelGGL(ff_dbias_kernel<TYPE>, dim3(cdiv(2LL * d->F, 32)), dim3(256), 0, s, *d, (const float*)sums, l.runs);
     VMM_LAUNCH_CHECK();
   }
+  if (!(d->dx && d->M > 0) && !d->dw_gate) return 0;
   Operands o;
   if (const int e = operands<TYPE>(d, l, o, s)) return e;
   const long long plane = d->M * l.fp;

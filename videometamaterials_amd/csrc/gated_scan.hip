@@ -14,7 +14,8 @@
 // What bounds it: memory, 3 values a step forward and 5 backward, plus 2 for the maps, which the third step finds in the 256 MB of last-level cache for
 // the most part: it walks time from the end, where step 1 has read last.  Passing states from workgroup to workgroup inside one launch would read all of
 // it once, and was built first; workgroups then poll each other's results past the caches, and 65536 steps of 1024 channels took 192 us (228 us
-// with groups and tiles of 128 steps; 370 us with tiles of 64) where these three launches take 0.17 ms.
+// with groups and tiles of 128 steps; 370 us with tiles of 64) where these three launches take 153 us (64 + 8 + 81;
+// the 402 MB that have to move once are 83 us of a copy).
 #include "vmm_common.h"
 #include "../../include/vmm_kernels.h"
 
@@ -139,7 +140,6 @@ __device__ __forceinline__ void gate_of(float g, float& f, float& i) {
   i = g < 0.f ? large : small;
 }
 
-typedef unsigned long long u64;
 struct ScanArgs {
   vmm_gated_scan_desc d;
   int tiles;           // of 64 channels
@@ -563,8 +563,12 @@ inline long long up16(long long n) { return (n + 15) / 16 * 16; }
 
 bool bad_rows(int64_t row) { return row < 0 || row >= (1LL << 23); }  // 64 rows are addressed with 32-bit byte offsets
 bool bad_scan(const vmm_gated_scan_desc* d) {
-  return !d || d->B < 0 || d->D < 0 || d->L < 0 || d->L >= (1LL << 31) || d->type < 0 || d->type > 2 || (int64_t)d->B * d->D >= (1LL << 31) ||
-         bad_rows(d->x_row) || bad_rows(d->gate_row) || bad_rows(d->y_row) || bad_rows(d->dy_row) || bad_rows(d->dx_row) || bad_rows(d->dgate_row);
+  if (!d || d->B < 0 || d->D < 0 || d->L < 0 || d->L >= (1LL << 31) || d->type < 0 || d->type > 2 || (int64_t)d->B * d->D >= (1LL << 31) ||
+         bad_rows(d->x_row) || bad_rows(d->gate_row) || bad_rows(d->y_row) || bad_rows(d->dy_row) || bad_rows(d->dx_row) || bad_rows(d->dgate_row))
+    return true;
+  // a launch has less than 2^32 threads: 256 a unit, 1024 a group
+  const long long chains = (long long)d->B * ((d->D + CG * V - 1) / (CG * V)), units = (d->L + UNIT - 1) / UNIT;
+  return chains * units > (1LL << 24) - 8 || (units > 1 && chains * ((units + GROUP - 1) / GROUP) > (1LL << 22) - 8);
 }
 
 struct Layout { unsigned units, groups; long long group_maps, anchors, states, bytes; };
@@ -617,7 +621,6 @@ int scan(const vmm_gated_scan_desc* d, bool forward, hipStream_t s) {
   a.units = l.units;
   a.groups = l.groups;
   a.runs = (d->x_row * esize(d->type)) % 128 != 0 || (d->gate_row * esize(d->type)) % 128 != 0;
-  if ((u64)l.units * d->B * a.tiles >= (1ull << 31)) return -1;
   char* w = (char*)d->workspace;
   a.maps = (float2*)w;
   a.group_maps = (float2*)(w + l.group_maps);

@@ -49,9 +49,9 @@ def _check_grads(tensors: Sequence[torch.Tensor], what: str) -> int:
 
 def _as_list(tensors, what: str) -> List[torch.Tensor]:
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{what}: expected tensors, got {type(t).__name__}")
+    for kind in set(map(type, tensors)):
+        if not issubclass(kind, torch.Tensor):
+            raise TypeError(f"{what}: expected tensors, got {kind.__name__}")
     return tensors
 
 
@@ -122,8 +122,8 @@ class ClippedAdam:
     """Adam (the update of torch.optim.Adam without weight decay or amsgrad) on gradients clipped by their global norm.
 
     params: float32 tensors, kept contiguous; exp_avgs / exp_avg_sqs: their moments (zeros where not given), step: the updates they have had.
-    max_norm None: no clipping.  The optimizer keeps one table of its tensors; ``step`` re-reads the addresses, so parameters may be re-homed
-    (``p.data = ...``) but not resized."""
+    max_norm None: no clipping.  The optimizer keeps one table of its tensors; ``step`` re-reads the parameters' addresses, so they may be re-homed
+    (``p.data = ...``) but not resized; the moments stay where they are: to load others, ``copy_`` into them."""
 
     def __init__(self, params: Iterable[torch.Tensor], lr: float = 1e-4, betas=(0.9, 0.999), eps: float = 1e-8, max_norm: Optional[float] = None, *,
                  exp_avgs: Optional[Iterable[torch.Tensor]] = None, exp_avg_sqs: Optional[Iterable[torch.Tensor]] = None, step: int = 0):
@@ -138,7 +138,8 @@ class ClippedAdam:
         self.exp_avgs = [torch.zeros_like(p, memory_format=torch.contiguous_format) for p in self.params] if exp_avgs is None else _as_list(exp_avgs, "ClippedAdam")
         self.exp_avg_sqs = [torch.zeros_like(p, memory_format=torch.contiguous_format) for p in self.params] if exp_avg_sqs is None \
             else _as_list(exp_avg_sqs, "ClippedAdam")
-        self.exp_avgs, self.exp_avg_sqs = [m.detach() for m in self.exp_avgs], [v.detach() for v in self.exp_avg_sqs]
+        self.exp_avgs, self.exp_avg_sqs = tuple(m.detach() for m in self.exp_avgs), tuple(v.detach() for v in self.exp_avg_sqs)
+        self._moments = (self.exp_avgs, self.exp_avg_sqs)  # the table below holds their addresses
         self._sizes = list(map(torch.Tensor.numel, self.params))
         for name, ts in (("params", self.params), ("exp_avgs", self.exp_avgs), ("exp_avg_sqs", self.exp_avg_sqs)):
             if len(ts) != len(self.params) or list(map(torch.Tensor.numel, ts)) != self._sizes:
@@ -151,7 +152,7 @@ class ClippedAdam:
         self._at: List[int] = []
 
     def _check_own(self) -> int:
-        every = self.params + self.exp_avgs + self.exp_avg_sqs
+        every = [*self.params, *self._moments[0], *self._moments[1]]
         if set(map(_dtype, every)) != {torch.float32}:
             raise TypeError("ClippedAdam: parameters and moments must be float32")
         if not all(map(torch.Tensor.is_contiguous, every)):
@@ -162,6 +163,8 @@ class ClippedAdam:
     def step(self, grads: Optional[Iterable[Optional[torch.Tensor]]] = None) -> torch.Tensor:
         """One update from `grads` (one per parameter; default: every ``p.grad``; None: that parameter stays as it is, and its moments too).
         Returns the gradients' global norm before clipping, a float32 scalar on the device."""
+        if torch.cuda.is_current_stream_capturing():  # (its replays would all be the same step)
+            raise RuntimeError("ClippedAdam.step: cannot be captured into a graph, the count of steps is the host's")
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"ClippedAdam.step: {len(grads)} gradients for {len(self.params)} parameters")

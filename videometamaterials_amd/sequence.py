@@ -25,8 +25,8 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """`t` with neighbouring values in its last dimension (a copy where they are not)."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 and t.is_contiguous() else t.contiguous()
+    """`t` with neighbouring values in its last dimension and rows less than 2^22 values apart, as the kernels' 32-bit offsets need them (else a copy)."""
+    return t if (t.stride(-1) == 1 or t.shape[-1] == 1 and t.is_contiguous()) and t.stride(-2) < 1 << 22 else t.contiguous()
 
 
 def _place(t: Optional[torch.Tensor]) -> tuple:
