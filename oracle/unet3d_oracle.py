@@ -51,6 +51,7 @@ class UnetCfg:
     cond_to_time: str = "add"
     per_frame_cond: bool = False
     padding_mode: str = "zeros"
+    cond_att_scan: bool = False  # (this package's own encoder: not in the reference)
     # derived (vddp.py:599-608)
     time_dim: int = field(init=False)
     cond_dim: int = field(init=False)
@@ -367,6 +368,23 @@ def signal_gru(sd, cond: Tensor) -> Tensor:
     return x
 
 
+def signal_scan(sd, cond: Tensor) -> Tensor:
+    """The encoder of Unet3D(cond_att_scan=True), step by step: per layer x, g = in_proj(s); h_t = f h_(t-1) + (1 - f) x_t with f = sigmoid(g_t);
+    s = h + down_proj(silu(gate_proj(h)) * up_proj(h))."""
+    s = cond[..., None]
+    for layer in range(3):
+        lin = lambda name, v: F.linear(v, sd[f"sign_emb_scan.layers.{layer}.{name}.weight"], sd[f"sign_emb_scan.layers.{layer}.{name}.bias"])  # noqa: E731
+        x, g = lin("in_proj", s).chunk(2, dim=-1)
+        h, outs = torch.zeros_like(x[:, 0]), []
+        for t in range(x.shape[1]):
+            f = torch.sigmoid(g[:, t])
+            h = f * h + (1 - f) * x[:, t]
+            outs.append(h)
+        y = torch.stack(outs, dim=1)
+        s = y + lin("down_proj", F.silu(lin("gate_proj", y)) * lin("up_proj", y))
+    return s
+
+
 def embed_condition(sd, cfg: UnetCfg, cond: Tensor, null_mask: Tensor):
     """vddp.py:751-795. Returns (tokens or None, hidden (B,time_dim))."""
     if cfg.per_frame_cond:
@@ -381,6 +399,8 @@ def embed_condition(sd, cfg: UnetCfg, cond: Tensor, null_mask: Tensor):
         if cfg.cond_attention != "none":
             if cfg.cond_att_GRU:
                 tokens = signal_gru(sd, cond)  # vddp.py:769-770: one token per sample of the conditioning signal (cond_attention_tokens == its length)
+            elif cfg.cond_att_scan:
+                tokens = signal_scan(sd, cond)
             else:
                 tokens = hidden[:, None, :].expand(-1, cfg.cond_attention_tokens, -1)
     if cfg.cond_attention != "none":

@@ -336,9 +336,15 @@ class DataParallelTrainer:
 
     def __init__(self, diffusion, *, train_lr: float = 1e-4, ema_decay: float = 0.995, step_start_ema: int = 2000, update_ema_every: int = 10,
                  null_cond_prob: float = 0.1, betas=(0.9, 0.999), eps: float = 1e-8, bucket_floats: int = 4_000_000, group=None,
-                 engine: Optional[str] = None):
+                 engine: Optional[str] = None, max_grad_norm: Optional[float] = None):
         """engine: "torch" = torch.distributed collectives (backend "nccl" is RCCL on ROCm; the default), "native" = the C-ABI engine of
-        include/vmm_dp.h (its own RCCL communicator and side stream; also at world 1).  Default: $VMM_DP_ENGINE or "torch"."""
+        include/vmm_dp.h (its own RCCL communicator and side stream; also at world 1).  Default: $VMM_DP_ENGINE or "torch".
+        max_grad_norm: the global norm that gradients are clipped to (None: no clipping) -- of the all-reduced, averaged and unscaled gradient, so every rank
+        takes the same factor; the optimizer launch applies it.  The norm of the last step is then `self.grad_norm` (a device scalar)."""
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError(f"max_grad_norm must be positive or None, got {max_grad_norm}")
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm: Optional[torch.Tensor] = None
         self.model = diffusion
         self.unet = diffusion.denoise_fn
         self.ema_model = copy.deepcopy(diffusion)  # vddp.py:1453
@@ -548,6 +554,10 @@ class DataParallelTrainer:
             j.p, j.m, j.n = p.data_ptr(), ema_params[name].data_ptr(), p.numel()
             self._max_n = max(self._max_n, p.numel())
         self._adam_table = (torch.frombuffer(bytearray(bytes(jobs)), dtype=torch.uint8).to(dev), len(jobs))
+        # the clipped step reads its jobs from the host; the gradients are one flat buffer (its padding stays zero)
+        self._clip_jobs = (N.ClipAdamJob * len(jobs))(*[N.ClipAdamJob(j.p, j.g, j.m, j.v, j.n, 0, 0) for j in jobs])
+        self._norm_job = N.GradJob(pl.pgrad.data_ptr(), pl.pgrad.numel(), 0, 0)
+        self._norm_work = torch.empty(N.lib().vmm_grad_norm_workspace(C.byref(self._norm_job), 1) // 8, dtype=torch.float64, device=dev)
         self._ema_table = (torch.frombuffer(bytearray(bytes(ejobs)), dtype=torch.uint8).to(dev), len(ejobs))
         self._ptr_sig = self._pointer_signature()
 
@@ -609,7 +619,18 @@ class DataParallelTrainer:
         self._reducer.finish()
         b1, b2 = self.betas
         tab, n = self._adam_table
-        if scaled:
+        if self.max_grad_norm is not None:
+            # norm and factor stay on the device; under loss scaling the same pass finds an inf / nan (vmm_grad_nonfinite below)
+            clip = torch.empty(2, dtype=torch.float32, device=dev)
+            state = st.data_ptr() if scaled else None
+            N.check(lib.vmm_grad_norm(C.byref(self._norm_job), 1, 1.0 / self.world, float(self.max_grad_norm), state, self._norm_work.data_ptr(), clip.data_ptr(),
+                                      _stream()), "vmm_grad_norm")
+            N.check(lib.vmm_adam_step_clipped(self._clip_jobs, len(self._clip_jobs), self.lr, b1, b2, self.eps, self.step, 1.0 / self.world, clip.data_ptr(), state,
+                                              _stream()), "vmm_adam_step_clipped")
+            if scaled:
+                N.check(lib.vmm_scaler_update(st.data_ptr(), self.loss_scale_growth, self.loss_scale_backoff, int(self.loss_scale_interval), _stream()), "vmm_scaler_update")
+            self.grad_norm = clip[0]
+        elif scaled:
             # GradScaler.step / update without a host round trip (vddp.py:1629-1633 under Accelerate's fp16): an inf / nan anywhere in the (all-reduced, hence
             # rank-consistent) gradient buffer turns the optimiser launch into a no-op and halves the scale; 2000 clean steps double it
             N.check(lib.vmm_grad_nonfinite(pl.pgrad.data_ptr(), pl.pgrad.numel(), st.data_ptr(), _stream()), "vmm_grad_nonfinite")

@@ -1507,6 +1507,71 @@ class _Builder:
                 max_x = max(max_x, j["rows"] * ((j["K"] + 63) // 64))
         self.step(self.lib.vmm_dense_bwd_batched, (self._upload_table(arr), len(jobs), max_n, max_x), what)
 
+    # ---------------------------------------------------------------- load-history encoder of gated linear recurrences (Unet3D(cond_att_scan=True))
+    SCAN_LAYERS = 3  # as many as the GRU encoder has (vddp.py:547)
+
+    def scan_encoder(self, cond_off: int) -> int:
+        """Three layers over the (B, L) signal, one token per sample of it: x, gate = in_proj(s); y = scan(x, gate); s = y + down(silu(gate_proj(y)) * up_proj(y)).
+        Returns the pointer of the last layer's rows [B][L][D]."""
+        lib, B, Lg, D = self.lib, self.B, self.cond_len, self.m.cond_dim
+        F = 2 * D
+        if Lg != self.ntok:
+            raise ValueError(f"cond_att_scan makes one token per sample of the conditioning signal: cond_attention_tokens ({self.ntok}) must equal its length ({Lg})")
+        xin, in_dim = self.ptr(cond_off), 1
+        self.scan_layers: List[dict] = []
+        for l in range(self.SCAN_LAYERS):
+            pf = f"sign_emb_scan.layers.{l}."
+            z, y, h, out = (self.ptr(self.alloc(B * Lg * n)) for n in (2 * D, D, F, D))
+            self.dense_level([dict(x=xin, w=self.wraw(pf + "in_proj.weight"), b=self.wraw(pf + "in_proj.bias"), y=z, rows=B * Lg, K=in_dim, N=2 * D)],
+                             f"sign_emb_scan layer {l}: candidates and gates")
+            scan = N.GatedScanDesc(x=z, x_batch=Lg * 2 * D, x_row=2 * D, gate=z + 4 * D, gate_batch=Lg * 2 * D, gate_row=2 * D, y=y, y_batch=Lg * D, y_row=D,
+                                   L=Lg, B=B, D=D)
+            if self.training:
+                scan.states = self.ptr(self.alloc(lib.vmm_gated_scan_states(C.byref(scan))))
+            scan.workspace = self.ptr(self.alloc((lib.vmm_gated_scan_workspace(C.byref(scan), 0) + 3) // 4 + 4))
+            self.step(lib.vmm_gated_scan, (C.byref(scan),), f"sign_emb_scan layer {l}: scan")
+            ff = N.GatedFFDesc(x=y, ldx=D, w_gate=self.wraw(pf + "gate_proj.weight"), w_up=self.wraw(pf + "up_proj.weight"), b_gate=self.wraw(pf + "gate_proj.bias"),
+                               b_up=self.wraw(pf + "up_proj.bias"), h=h, ldh=F, M=B * Lg, K=D, F=F)
+            if self.training:
+                ff.g_pre, ff.u_pre = self.ptr(self.alloc(B * Lg * F)), self.ptr(self.alloc(B * Lg * F))
+            ff.workspace = self.ptr(self.alloc((lib.vmm_gated_ff_workspace(C.byref(ff), 0) + 3) // 4 + 4))
+            self.step(lib.vmm_gated_ff, (C.byref(ff),), f"sign_emb_scan layer {l}: gated feed-forward", flops=4.0 * B * Lg * D * F)
+            self.dense_level([dict(x=h, w=self.wraw(pf + "down_proj.weight"), b=self.wraw(pf + "down_proj.bias"), add=y, ldadd=D, y=out, rows=B * Lg, K=F, N=D)],
+                             f"sign_emb_scan layer {l}: back to the width, plus the states")
+            for nm_ in ("in_proj", "gate_proj", "up_proj", "down_proj"):
+                self._touch(pf + nm_ + ".weight")
+                self._touch(pf + nm_ + ".bias")
+            self.scan_layers.append(dict(pf=pf, x=xin, in_dim=in_dim, z=z, y=y, h=h, scan=scan, ff=ff))
+            xin, in_dim = out, D
+        return xin
+
+    def scan_encoder_bwd(self, dout: int) -> None:
+        """Backward of scan_encoder from the gradient of its last rows."""
+        lib, B, Lg, D = self.lib, self.B, self.cond_len, self.m.cond_dim
+        F, n = 2 * D, B * Lg * D
+        pg = lambda name: self.pg(name) or self.scratch(int(math.prod(self.shapes[name])))  # noqa: E731 (a frozen parameter's gradient goes nowhere)
+        for l in reversed(range(self.SCAN_LAYERS)):
+            s = self.scan_layers[l]
+            pf, scan, ff = s["pf"], s["scan"], s["ff"]
+            dh = self.scratch(B * Lg * F)  # (zeroed every backward: the dense backward accumulates into it)
+            self.dense_bwd_level([dict(x=s["h"], w=self.wraw(pf + "down_proj.weight"), dy=dout, dx=dh, dw=self.pg(pf + "down_proj.weight"),
+                                       db=self.pg(pf + "down_proj.bias"), rows=B * Lg, K=F, N=D)], f"sign_emb_scan layer {l}: down_proj bwd")
+            dy, dz = self.ptr(self.alloc(n)), self.ptr(self.alloc(2 * n))
+            fb = N.GatedFFDesc(x=ff.x, ldx=D, w_gate=ff.w_gate, w_up=ff.w_up, g_pre=ff.g_pre, u_pre=ff.u_pre, dh=dh, lddh=F, dx=dy, lddx=D, dw_gate=pg(pf + "gate_proj.weight"),
+                               dw_up=pg(pf + "up_proj.weight"), db_gate=pg(pf + "gate_proj.bias"), db_up=pg(pf + "up_proj.bias"), M=B * Lg, K=D, F=F)
+            fb.workspace = self.ptr(self.alloc((lib.vmm_gated_ff_workspace(C.byref(fb), 1) + 3) // 4 + 4))
+            self.step(lib.vmm_gated_ff_bwd, (C.byref(fb),), f"sign_emb_scan layer {l}: gated feed-forward bwd", flops=8.0 * B * Lg * D * F)
+            self.step(lib.vmm_lincomb, (dout, dy, None, 1.0, 1.0, 0.0, 0.0, dy, n), f"sign_emb_scan layer {l}: gradient of the states")
+            sb = N.GatedScanDesc(x=scan.x, x_batch=scan.x_batch, x_row=scan.x_row, gate=scan.gate, gate_batch=scan.gate_batch, gate_row=scan.gate_row, states=scan.states,
+                                 dy=dy, dy_batch=Lg * D, dy_row=D, dx=dz, dx_batch=Lg * 2 * D, dx_row=2 * D, dgate=dz + 4 * D, dgate_batch=Lg * 2 * D,
+                                 dgate_row=2 * D, L=Lg, B=B, D=D)
+            sb.workspace = self.ptr(self.alloc((lib.vmm_gated_scan_workspace(C.byref(sb), 1) + 3) // 4 + 4))
+            self.step(lib.vmm_gated_scan_bwd, (C.byref(sb),), f"sign_emb_scan layer {l}: scan bwd")
+            dx = self.scratch(B * Lg * s["in_dim"]) if l > 0 else 0
+            self.dense_bwd_level([dict(x=s["x"], w=self.wraw(pf + "in_proj.weight"), dy=dz, dx=dx, dw=self.pg(pf + "in_proj.weight"), db=self.pg(pf + "in_proj.bias"),
+                                       rows=B * Lg, K=s["in_dim"], N=2 * D)], f"sign_emb_scan layer {l}: in_proj bwd")
+            dout = dx
+
     def emit_unpack(self, jobs: List[dict], what: str) -> None:
         """Scatter packed weight gradients into the flat torch-layout gradient buffer (one batched launch)."""
         if not jobs:
@@ -1638,6 +1703,9 @@ class _Builder:
                     gru.append((xin, in_dim, wih, whh, bih, bhh, hp, gates))
                     xin, in_dim = self.ptr(yl), D
                 self.step(lib.vmm_tokens_select, (xin, self.wraw("null_text_token"), self.ptr(mask_off), B, ntok, D, self.ptr(tokens)), "tokens (GRU states)")
+            elif tokens is not None and getattr(m, "cond_att_scan", False):
+                self.step(lib.vmm_tokens_select, (self.scan_encoder(cond_off), self.wraw("null_text_token"), self.ptr(mask_off), B, ntok, D, self.ptr(tokens)),
+                          "tokens (scanned states)")
             elif tokens is not None:
                 self.step(lib.vmm_tokens_from_hidden, (self.ptr(hidden), self.wraw("null_text_token"), self.ptr(mask_off), B, ntok, D, self.ptr(tokens)), "tokens")
             if tr:
@@ -1655,6 +1723,10 @@ class _Builder:
                                                   dict(x=hp, w=self.wraw(whh), dy=dgh, dw=self.pg(whh), db=self.pg(bhh), rows=B * Lg, K=D, N=3 * D)],
                                                  f"sign_emb_GRU layer {l}: weight / bias / input gradients")
                             dy = dx
+                    elif tokens is not None and getattr(m, "cond_att_scan", False):
+                        dy = self.ptr(self.alloc(B * ntok * D))
+                        self.step(lib.vmm_tokens_select_bwd, (self.dtokens_ptr, self.ptr(mask_off), B, ntok, D, dy, self.pg("null_text_token")), "tokens bwd")
+                        self.scan_encoder_bwd(dy)
                     elif tokens is not None:
                         self.step(lib.vmm_tokens_from_hidden_bwd, (self.dtokens_ptr, self.ptr(mask_off), B, ntok, D, ghidden, self.pg("null_text_token")),
                                   "tokens bwd")

@@ -70,6 +70,7 @@ class Unet3D(nn.Module):
         cond_to_time="add",
         per_frame_cond=False,
         padding_mode="zeros",
+        cond_att_scan=False,
     ):
         super().__init__()
         assert init_kernel_size % 2 == 1  # vddp.py:621
@@ -90,6 +91,11 @@ class Unet3D(nn.Module):
         if self.cond_attention not in ("none", "self-stacked", "cross-attention"):
             raise ValueError("cond_attention must be none, self-stacked or cross-attention")
         self.cond_att_GRU = cond_att_GRU
+        # cond_att_scan (not in the reference; beside its cond_att_GRU): the conditioning tokens are the states of three gated linear recurrences over the
+        # signal, each with a gated feed-forward behind it (sequence.py) -- scanned in parallel over time where the GRU walks it step by step
+        if cond_att_scan and (cond_att_GRU or per_frame_cond or cond_attention == "none"):
+            raise ValueError("cond_att_scan makes the attention tokens from the conditioning signal: not with cond_att_GRU, per_frame_cond or cond_attention='none'")
+        self.cond_att_scan = cond_att_scan
         self.cond_dim = self.time_dim
         self.use_temporal_attention_cond = use_temporal_attention_cond
         self.cond_to_time = cond_to_time
@@ -201,6 +207,15 @@ class Unet3D(nn.Module):
             for l in range(3):
                 for nm_, shp in (("weight_ih", (3 * cd, 1 if l == 0 else cd)), ("weight_hh", (3 * cd, cd)), ("bias_ih", (3 * cd,)), ("bias_hh", (3 * cd,))):
                     _attach(self, f"sign_emb_GRU.emb_model.{nm_}_l{l}", _uniform(shp, cd))
+        if self.cond_att_scan:
+            for l in range(_plan._Builder.SCAN_LAYERS):
+                p = f"sign_emb_scan.layers.{l}."
+                self._linear(p + "in_proj", 2 * cd, 1 if l == 0 else cd)  # candidates, then gates
+                with torch.no_grad():  # forget gates from a memory of two samples to one of some fifty, channel by channel
+                    self.get_parameter(p + "in_proj.bias")[cd:] += torch.linspace(0.0, 4.0, cd)
+                self._linear(p + "gate_proj", 2 * cd, cd)
+                self._linear(p + "up_proj", 2 * cd, cd)
+                self._linear(p + "down_proj", cd, 2 * cd)
         if self.per_frame_cond:
             self._linear("sign_emb", cd, 1)
             _attach(self, "cond_token_to_hidden.0.weight", torch.ones(cd))
