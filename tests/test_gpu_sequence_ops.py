@@ -609,6 +609,59 @@ def test_captured_operators_replay(gpu):
             assert all(torch.equal(p, q) for p, q in zip(out, want)) and all(torch.equal(p, q) for p, q in zip(grads, new)), (turn, k)
 
 
+def test_captured_training_pass_replays(gpu):
+    """Forward and backward of the operators in one graph, replayed on new inputs with eager passes between, while an eager graph of the same tensors lives."""
+    args = layer_inputs(gpu, torch.bfloat16, 7)
+    from videometamaterials_amd import gated_linear_scan
+    alive = gated_linear_scan(args[0].clone().requires_grad_(), args[1])
+    s = torch.cuda.Stream(gpu)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        everything(*args)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = everything(*args)
+    for turn in range(4):
+        fresh = layer_inputs(gpu, torch.bfloat16, 20 + turn)
+        for a, f in zip(args, fresh):
+            a.copy_(f)
+        graph.replay()
+        want = everything(*fresh)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want)), turn
+    assert bool(torch.isfinite(alive[0]).all())
+
+
+def test_gradients_are_differentiable_once_and_saved_tensors_are_watched(gpu):
+    from videometamaterials_amd import gated_feed_forward, gated_linear_scan
+    x, gate, w = (torch.randn(*s, device=gpu, requires_grad=True) for s in ((2, 70, 16), (2, 70, 16), (8, 16)))
+    for value, leaf in ((lambda: gated_linear_scan(x, gate)[0], gate), (lambda: gated_feed_forward(x, w, w), w)):
+        y = value()
+        d = torch.autograd.grad(y, leaf, torch.ones_like(y), create_graph=True)[0]
+        assert torch.equal(d.detach(), torch.autograd.grad(value(), leaf, torch.ones_like(y))[0])
+        with pytest.raises(RuntimeError):
+            d.sum().backward()
+        y = value()
+        with torch.no_grad():
+            leaf.mul_(1.0)
+        with pytest.raises(RuntimeError):
+            y.sum().backward()
+
+
+def test_clipped_adam_is_not_captured(gpu):
+    from videometamaterials_amd import ClippedAdam
+    p = torch.ones(100, device=gpu)
+    opt, g, scratch = ClippedAdam([p]), torch.ones(100, device=gpu), torch.zeros(4, device=gpu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        scratch.add_(1.0)
+        with pytest.raises(RuntimeError):
+            opt.step([g])
+    graph.replay()
+    assert opt.steps_taken == 0 and float(p.sum()) == 100.0 and float(scratch[0]) == 1.0
+
+
 def test_training_an_encoder_layer_with_all_of_them(gpu):
     """A layer of projection, scan and gated feed-forward, trained for some steps by the clipped optimizer, against the same layer of torch operations with
     clip_grad_norm_ and torch.optim.Adam: the weights stay together (both take the same ten steps of 1e-3; a step's relative error is that of its gradient)."""

@@ -13,7 +13,6 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 def test_structs_match_the_header(tmp_path):
     from videometamaterials_amd import _native as N
-    from videometamaterials_amd import optim as O
     if shutil.which("gcc") is None:
         pytest.skip("no gcc")
     pairs = {"vmm_gated_scan_desc": N.GatedScanDesc, "vmm_gated_ff_desc": N.GatedFFDesc, "vmm_grad_job": N.GradJob, "vmm_clip_adam_job": N.ClipAdamJob}
@@ -32,8 +31,6 @@ def test_structs_match_the_header(tmp_path):
         assert all(int(got[f"{name}.{f}"]) == getattr(cls, f).offset for f, _ in cls._fields_)
         body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), hdr, flags=re.S).group(1), flags=re.S)
         assert len([m for decl in body.split(";") for m in decl.split(",") if m.strip()]) == len(cls._fields_)
-    for cls, rows in ((N.GradJob, O.GRAD_JOB), (N.ClipAdamJob, O.ADAM_JOB)):  # the arrays that the optimizer fills in column by column
-        assert rows.itemsize == C.sizeof(cls) and all(rows.fields[n][1] == getattr(cls, n).offset for n in rows.names)
 
 
 def test_bad_descriptors_are_refused_before_any_launch():

@@ -418,6 +418,23 @@ def lib() -> C.CDLL:
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The compiled torch layer of the sequence operators (csrc/torch_binding.cpp), bound to the loaded library; raises if it has not been built."""
+    global _binding
+    if _binding is None:
+        handle = lib()
+        try:
+            from . import _sequence
+        except ImportError as e:
+            raise NativeError(f"the torch layer of the sequence operators is missing: build it (python -m videometamaterials_amd.build): {e}") from e
+        _sequence.bind({name: C.cast(getattr(handle, name), C.c_void_p).value for name in _sequence.entries})
+        _binding = _sequence
+    return _binding
+
+
 def experiments_built() -> bool:
     """True when the loaded library is the experiments build (libvmm_hip_exp.so via VMM_LIB_PATH)."""
     return all(hasattr(lib(), name) for name in EXPERIMENT_SIGNATURES)

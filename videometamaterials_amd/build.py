@@ -19,6 +19,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 EXPERIMENTS = os.environ.get("VMM_EXPERIMENTS", "0") not in ("", "0")
 OUT = os.path.join(HERE, "libvmm_hip_exp.so" if EXPERIMENTS else "libvmm_hip.so")
+BINDING = os.path.join(CSRC, "torch_binding.cpp")
+BINDING_OUT = os.path.join(HERE, "_sequence.so")
 OBJDIR = os.path.join(HERE, "_obj_exp" if EXPERIMENTS else "_obj")
 EXPERIMENT_SOURCES = {"conv3x3_wino.hip"}
 # compiled a second time with -DVMM_SINGLE_PASS=1 (object *_sp.o): the `_bf16` entry points of the backward kernels (vmm_common.h, VMM_X3)
@@ -109,7 +111,29 @@ def build(force: bool = False, verbose: bool = True) -> str:
         if res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
             raise RuntimeError("link failed")
+    if not EXPERIMENTS:
+        _build_binding(force, verbose)
     return OUT
+
+
+def _build_binding(force: bool, verbose: bool) -> None:
+    """_sequence.so: the torch layer of the sequence operators, host code alone; the C ABI it calls is handed to it at run time."""
+    import sysconfig
+    import torch
+    inc = [os.path.join(os.path.dirname(torch.__file__), *p) for p in (("include",), ("include", "torch", "csrc", "api", "include"))]
+    inc += [os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           *[f for i in inc for f in ("-isystem", i)], BINDING, "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python",
+           "-lc10_hip", "-o", BINDING_OUT]
+    if force or _stale(BINDING_OUT, [BINDING] + glob.glob(os.path.join(HERE, "..", "include", "*.h"))) or _flags_changed(cmd):
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if verbose:
+            print("g++ torch_binding.cpp")
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError("g++ failed on torch_binding.cpp")
+        with open(cmd[-1] + ".cmd", "w") as f:
+            f.write(" ".join(cmd))
 
 
 if __name__ == "__main__":
