@@ -31,7 +31,7 @@ template <int TYPE> struct Elem;
 template <> struct Elem<0> { typedef float T; typedef uint4 W; static constexpr unsigned PAD = 0x42D00000u; };
 template <> struct Elem<1> { typedef __bf16 T; typedef uint2 W; static constexpr unsigned PAD = 0x42D042D0u; };
 template <> struct Elem<2> { typedef _Float16 T; typedef uint2 W; static constexpr unsigned PAD = 0x56805680u; };
-// PAD: gates of 104.  sigmoid(104) is 1 in fp32, so a padded step (x = 0) is the identity map, and its 1 - f is below the smallest normal number.
+// PAD: gates of 104.  sigmoid(104) is 1 in fp32, so a padded step (x = 0) is the identity map.
 
 // V values side by side, kept as loaded until they are used
 template <int TYPE> struct Raw {
@@ -119,25 +119,29 @@ struct Place {
 // a value that is the same in every lane, in a scalar register
 __device__ __forceinline__ unsigned uniform(unsigned v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// f = sigmoid(g) and i = 1 - f = sigmoid(-g), each accurate in itself: e = exp(-|g|), the smaller of the two is e / (1 + e), the larger 1 minus that, with
-// one rounding -- a gate close to one is multiplied with itself over a whole memory, where the error of a reciprocal would add up.  fp32 gates correct
-// exp for what rounding p = -|g| log2(e) has lost, up to |g| 2^-25 of e; 16-bit gates are themselves rounded by more than that.  NaN passes.
+// f = sigmoid(g) and i = 1 - f = sigmoid(-g).  These kernels are bound by their instructions as much as by memory, and the gate is a third of them.
+// 16 bits: i = 1 / (1 + e^g), f = 1 - i, whatever e^g is, zero and infinite too.  The gates that are multiplied with themselves over a whole memory, f near
+// one, have one rounding -- the error of a reciprocal would add up there; f near zero is off by a rounding of one, as its products with states and
+// inputs of one's size are anyway.
+// fp32: each accurate in itself.  e = exp(-|g|), the smaller of the two is e / (1 + e), the larger 1 minus that; exp is corrected for what rounding
+// p = -|g| log2(e) has lost, up to |g| 2^-25 of e.  NaN passes in both.
 template <int TYPE>
 __device__ __forceinline__ void gate_of(float g, float& f, float& i) {
-  float e, m = fabsf(g);
   if constexpr (TYPE == 0) {
+    float m = fabsf(g);
     m = m > 104.f ? 104.f : m;  // (exp is zero from there on; an infinite one would leave inf - inf below)
     const float p = m * -1.44269502162933349609375f;
     float t = fmaf(m, -1.44269502162933349609375f, -p);
     t = fmaf(m, -1.925963033500011e-08f, t);
-    e = __builtin_amdgcn_exp2f(p);
+    float e = __builtin_amdgcn_exp2f(p);
     e = fmaf(e, t * 0.6931471805599453f, e);
+    const float small = e * __builtin_amdgcn_rcpf(1.0f + e), large = 1.0f - small;
+    f = g < 0.f ? small : large;
+    i = g < 0.f ? large : small;
   } else {
-    e = __builtin_amdgcn_exp2f(m * -1.44269502162933349609375f);
+    i = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * 1.44269502162933349609375f));
+    f = 1.0f - i;
   }
-  const float small = e * __builtin_amdgcn_rcpf(1.0f + e), large = 1.0f - small;
-  f = g < 0.f ? small : large;
-  i = g < 0.f ? large : small;
 }
 
 struct ScanArgs {

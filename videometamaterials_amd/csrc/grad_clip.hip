@@ -126,6 +126,7 @@ __global__ __launch_bounds__(256) void grad_square_kernel(const GradTable t, dou
 __global__ __launch_bounds__(256) void grad_norm_finish_kernel(const double* __restrict__ partial, int n, float scale, float max_norm, float* __restrict__ scaler,
                                                                float* __restrict__ out) {
   double s = 0.0;
+#pragma unroll 8
   for (int i = threadIdx.x; i < n; i += 256) s += partial[i];
   s = block_sum(s);
   if (threadIdx.x == 0) {
