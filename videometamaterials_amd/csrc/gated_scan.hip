@@ -11,11 +11,12 @@
 // A sequence of one unit needs the last alone.  Where there are more than 256 groups, the state in front of every 256th (an anchor) is formed first, so
 // that step 2 goes through 255 groups at the most.  Which maps are joined in which order depends on the sizes alone: the same bits every time.
 //
-// What bounds it: memory, 3 values a step forward and 5 backward, plus 2 for the maps, which the third step finds in the 256 MB of last-level cache for
-// the most part: it walks time from the end, where step 1 has read last.  Passing states from workgroup to workgroup inside one launch would read all of
-// it once, and was built first; workgroups then poll each other's results past the caches, and 65536 steps of 1024 channels took 192 us (228 us
-// with groups and tiles of 128 steps; 370 us with tiles of 64) where these three launches take 153 us (64 + 8 + 81;
-// the 402 MB that have to move once are 83 us of a copy).
+// What bounds it: memory and instructions alike.  3 values a step move forward and 5 backward, plus 2 for the maps, which the third step finds in the 256 MB
+// of last-level cache for the most part: it walks time from the end, where step 1 has read last.  65536 steps of 1024 channels in bf16 take 56 + 8 + 69 us: the
+// maps read at a copy's 4.8 TB/s; the 402 MB that have to move once are 83 us of it.  Each value costs some thirty instructions, so whatever can be
+// decided for a whole unit is (see `unit`).  Passing states from workgroup to workgroup inside one launch would read all of it once, and was
+// built first; workgroups then poll each other's results past the caches, and the same took 192 us (228 us with groups and tiles of 128 steps; 370 us with tiles of 64).
+#include <type_traits>
 #include "vmm_common.h"
 #include "../../include/vmm_kernels.h"
 
@@ -214,82 +215,92 @@ __global__ __launch_bounds__(1024) void scan_map_kernel(const ScanArgs a) {
   const unsigned id = number(a, a.groups * d.B * a.tiles);
   if (id >= a.groups * d.B * a.tiles) return;
   const unsigned rest = uniform(id / a.tiles), tile = id - rest * a.tiles, group = uniform(rest / d.B), b = rest - group * d.B;
-  const Place<TYPE, WIDE> at(cg, d.D - (int)tile * CG * V);
+  const int columns = d.D - (int)tile * CG * V;
   const unsigned u = group * GROUP + wave;  // in the direction of the walk
   const bool exists = u < a.units;
   const long long first = (long long)(BACK ? a.units - 1 - u : u) * UNIT;
   long long len = d.L;
   if (d.lengths) len = max(0LL, min((long long)d.lengths[b], len));
-  const int live = exists ? (int)min(max(len - first, 0LL), (long long)UNIT) - quarter * STEPS : 0;
   const long long es = sizeof(typename Elem<TYPE>::T), bd = (long long)b * d.D + (long long)tile * CG * V;
   const void* xv = BACK ? d.dy : d.x;
   const int64_t xb = BACK ? d.dy_batch : d.x_batch, xs = BACK ? d.dy_row : d.x_row;
   const auto row = [&](const void* p, int64_t batch, int64_t step, int k) {
     return (const char*)p + (b * batch + (first + k) * step + (long long)tile * CG * V) * es;
   };
-  const unsigned xl = (quarter * STEPS * (unsigned)xs + at.d0) * (unsigned)es, gl = (quarter * STEPS * (unsigned)d.gate_row + at.d0) * (unsigned)es;
   const bool has_x = !BACK || d.dy;
-  Raw<TYPE> x[BATCH], g[BATCH];
-  auto load = [&](int k0) {
+  const auto unit = [&](auto whole) {
+    constexpr bool ALL = decltype(whole)::value;
+    const Place<TYPE, WIDE> at(cg, ALL ? CG * V : columns);
+    const int live = ALL ? UNIT : exists ? (int)min(max(len - first, 0LL), (long long)UNIT) - quarter * STEPS : 0;
+    const unsigned xl = (quarter * STEPS * (unsigned)xs + at.d0) * (unsigned)es, gl = (quarter * STEPS * (unsigned)d.gate_row + at.d0) * (unsigned)es;
+    Raw<TYPE> x[BATCH], g[BATCH];
+    auto load = [&](int k0) {
 #pragma unroll
-    for (int k = 0; k < BATCH; ++k) {
-      x[k].u = fill_word<TYPE>(0u);
-      g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
-      if (k0 + k < live) {
-        if (has_x) x[k].u = at.load(row(xv, xb, xs, k0 + k), xl, 0u);
-        g[k].u = at.load(row(d.gate, d.gate_batch, d.gate_row, k0 + k), gl, Elem<TYPE>::PAD);
+      for (int k = 0; k < BATCH; ++k) {
+        x[k].u = fill_word<TYPE>(0u);
+        g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
+        if (k0 + k < live) {
+          if (has_x) x[k].u = at.load(row(xv, xb, xs, k0 + k), xl, 0u);
+          g[k].u = at.load(row(d.gate, d.gate_batch, d.gate_row, k0 + k), gl, Elem<TYPE>::PAD);
+        }
+      }
+    };
+    float P[V], Q[V], pe[V], qe[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; }
+    if (ALL || (exists && len > first)) {
+      load(BACK ? STEPS - BATCH : 0);
+#pragma unroll
+      for (int n = 0; n < BATCHES; ++n) {
+        float f[BATCH][V], q[BATCH][V];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            float i;
+            gate_of<TYPE>(g[k].get(j), f[k][j], i);
+            q[k][j] = BACK ? x[k].get(j) : i * x[k].get(j);
+          }
+        if (n + 1 < BATCHES) load((BACK ? BATCHES - 2 - n : n + 1) * BATCH);
+#pragma unroll
+        for (int s = 0; s < BATCH; ++s) {
+          const int k = BACK ? BATCH - 1 - s : s;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            Q[j] = BACK ? f[k][j] * (q[k][j] + Q[j]) : fmaf(f[k][j], Q[j], q[k][j]);
+            P[j] *= f[k][j];
+          }
+        }
+      }
+    }
+    wave_join<!BACK>(P, Q, pe, qe);
+    if (quarter == 0) {
+      float2* m = a.maps + (long long)u * d.B * d.D + bd;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        join[wave][cg][j] = make_float2(P[j], Q[j]);
+        if (exists && at.has(j)) m[at.channel(j)] = make_float2(P[j], Q[j]);
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < 16) {
+      float2* gm = a.group_maps + (long long)group * d.B * d.D + bd;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float p = 1.f, q = 0.f;
+        for (int r = 0; r < GROUP; ++r) {  // (units that do not exist left the identity)
+          const float2 w = join[r][cg][j];
+          p *= w.x;
+          q = fmaf(w.x, q, w.y);
+        }
+        if (at.has(j)) gm[at.channel(j)] = make_float2(p, q);
       }
     }
   };
-  float P[V], Q[V], pe[V], qe[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; }
-  load(BACK ? STEPS - BATCH : 0);
-#pragma unroll
-  for (int n = 0; n < BATCHES; ++n) {
-    float f[BATCH][V], q[BATCH][V];
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float i;
-        gate_of<TYPE>(g[k].get(j), f[k][j], i);
-        q[k][j] = BACK ? x[k].get(j) : i * x[k].get(j);
-      }
-    if (n + 1 < BATCHES) load((BACK ? BATCHES - 2 - n : n + 1) * BATCH);
-#pragma unroll
-    for (int s = 0; s < BATCH; ++s) {
-      const int k = BACK ? BATCH - 1 - s : s;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        Q[j] = BACK ? f[k][j] * (q[k][j] + Q[j]) : fmaf(f[k][j], Q[j], q[k][j]);
-        P[j] *= f[k][j];
-      }
-    }
-  }
-  wave_join<!BACK>(P, Q, pe, qe);
-  if (quarter == 0) {
-    float2* m = a.maps + (long long)u * d.B * d.D + bd;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      join[wave][cg][j] = make_float2(P[j], Q[j]);
-      if (exists && at.has(j)) m[at.channel(j)] = make_float2(P[j], Q[j]);
-    }
-  }
-  __syncthreads();
-  if (threadIdx.x < 16) {
-    float2* gm = a.group_maps + (long long)group * d.B * d.D + bd;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float p = 1.f, q = 0.f;
-      for (int r = 0; r < GROUP; ++r) {  // (units that do not exist left the identity)
-        const float2 w = join[r][cg][j];
-        p *= w.x;
-        q = fmaf(w.x, q, w.y);
-      }
-      if (at.has(j)) gm[at.channel(j)] = make_float2(p, q);
-    }
-  }
+  // Nearly every group is whole (all steps within the length, all channels there), and works without masks, paddings and their moves: 85 -> 69 us for the
+  // application and 59 -> 56 for the maps of 65536 x 1024.  (A third form, for units behind a sequence's end, gained nothing.)
+  if (columns >= CG * V && (group + 1) * GROUP <= a.units && len >= (BACK ? a.units - group * GROUP : (group + 1) * GROUP) * (long long)UNIT && has_x) unit(std::true_type{});
+  else unit(std::false_type{});
 }
 
 // ---- step 2.  16 lanes of 4 channels x 16 rows a workgroup, as above; channels side by side (maps and states are the kernels' own: always aligned to
@@ -395,67 +406,73 @@ __global__ __launch_bounds__(256, 5) void scan_fwd_kernel(const ScanArgs a) {
   const unsigned rest = uniform(id / a.tiles), tile = id - rest * a.tiles, turn = uniform(rest / d.B), b = rest - turn * d.B;
   const unsigned u = a.units - 1 - turn;  // from the end of time, where the maps were read last
   const long long first = (long long)u * UNIT;
-  const Place<TYPE, WIDE> at(cg, d.D - (int)tile * CG * V);
+  const int columns = d.D - (int)tile * CG * V;
   long long len = d.L;
   if (d.lengths) len = max(0LL, min((long long)d.lengths[b], len));
-  const int live = (int)min(max(len - first, 0LL), (long long)UNIT) - seg * TS, there = (int)min(d.L - first, (int64_t)UNIT) - seg * TS;
   const long long es = sizeof(typename Elem<TYPE>::T), bd = (long long)b * d.D + (long long)tile * CG * V;
   const auto row = [&](auto* p, int64_t batch, int64_t step, int k) { return p + (b * batch + (first + k) * step + (long long)tile * CG * V) * es; };
-  const auto lane = [&](int64_t step) { return (seg * TS * (unsigned)step + at.d0) * (unsigned)es; };
-  Raw<TYPE> x[TS], g[TS];
-  const unsigned xl = lane(d.x_row), gl = lane(d.gate_row);
+  const auto unit = [&](auto whole) {
+    constexpr bool ALL = decltype(whole)::value;
+    const Place<TYPE, WIDE> at(cg, ALL ? CG * V : columns);
+    const int live = ALL ? UNIT : (int)min(max(len - first, 0LL), (long long)UNIT) - seg * TS, there = ALL ? UNIT : (int)min(d.L - first, (int64_t)UNIT) - seg * TS;
+    const auto lane = [&](int64_t step) { return (seg * TS * (unsigned)step + at.d0) * (unsigned)es; };
+    Raw<TYPE> x[TS], g[TS];
+    const unsigned xl = lane(d.x_row), gl = lane(d.gate_row);
 #pragma unroll
-  for (int k = 0; k < TS; ++k) {
-    x[k].u = fill_word<TYPE>(0u);
-    g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
-    if (k < live) {
-      x[k].u = at.load(row((const char*)d.x, d.x_batch, d.x_row, k), xl, 0u);
-      g[k].u = at.load(row((const char*)d.gate, d.gate_batch, d.gate_row, k), gl, Elem<TYPE>::PAD);
+    for (int k = 0; k < TS; ++k) {
+      x[k].u = fill_word<TYPE>(0u);
+      g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
+      if (k < live) {
+        x[k].u = at.load(row((const char*)d.x, d.x_batch, d.x_row, k), xl, 0u);
+        g[k].u = at.load(row((const char*)d.gate, d.gate_batch, d.gate_row, k), gl, Elem<TYPE>::PAD);
+      }
     }
-  }
-  float h[V];
+    float h[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) h[j] = 0.f;
-  if (a.units > 1) at.load_state(a.states + (long long)u * d.B * d.D + bd, h);
-  else if (d.h0) at.load_state(d.h0 + bd, h);
-  if (a.units == 1 && d.states && seg == 0) at.store_state(d.states + bd, h);  // (step 2 would have left it)
+    for (int j = 0; j < V; ++j) h[j] = 0.f;
+    if (a.units > 1) at.load_state(a.states + (long long)u * d.B * d.D + bd, h);
+    else if (d.h0) at.load_state(d.h0 + bd, h);
+    if (a.units == 1 && d.states && seg == 0) at.store_state(d.states + bd, h);  // (step 2 would have left it)
 
-  float f[TS][V], q[TS][V], P[V], Q[V], pe[V], qe[V];
+    float f[TS][V], q[TS][V], P[V], Q[V], pe[V], qe[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; }
+    for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; }
 #pragma unroll
-  for (int k = 0; k < TS; ++k)
+    for (int k = 0; k < TS; ++k)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float i;
-      gate_of<TYPE>(g[k].get(j), f[k][j], i);
-      q[k][j] = i * x[k].get(j);
-      P[j] *= f[k][j];
-      Q[j] = fmaf(f[k][j], Q[j], q[k][j]);
+      for (int j = 0; j < V; ++j) {
+        float i;
+        gate_of<TYPE>(g[k].get(j), f[k][j], i);
+        q[k][j] = i * x[k].get(j);
+        P[j] *= f[k][j];
+        Q[j] = fmaf(f[k][j], Q[j], q[k][j]);
+      }
+    wave_join<true>(P, Q, pe, qe);
+    if ((threadIdx.x & 48) == 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) wave_map[wave][cg][j] = make_float2(P[j], Q[j]);
     }
-  wave_join<true>(P, Q, pe, qe);
-  if ((threadIdx.x & 48) == 0) {
+    __syncthreads();  // (and every wave has read h0, which h_last may be)
+    for (int w = 0; w < wave; ++w)
 #pragma unroll
-    for (int j = 0; j < V; ++j) wave_map[wave][cg][j] = make_float2(P[j], Q[j]);
-  }
-  __syncthreads();  // (and every wave has read h0, which h_last may be)
-  for (int w = 0; w < wave; ++w)
+      for (int j = 0; j < V; ++j) h[j] = fmaf(wave_map[w][cg][j].x, h[j], wave_map[w][cg][j].y);
 #pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = fmaf(wave_map[w][cg][j].x, h[j], wave_map[w][cg][j].y);
+    for (int j = 0; j < V; ++j) h[j] = fmaf(pe[j], h[j], qe[j]);
+    const unsigned yl = lane(d.y_row);
 #pragma unroll
-  for (int j = 0; j < V; ++j) h[j] = fmaf(pe[j], h[j], qe[j]);
-  const unsigned yl = lane(d.y_row);
+    for (int k = 0; k < TS; ++k) {
+      float o[V];
 #pragma unroll
-  for (int k = 0; k < TS; ++k) {
-    float o[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      h[j] = fmaf(f[k][j], h[j], q[k][j]);
-      o[j] = k < live ? h[j] : 0.f;
+      for (int j = 0; j < V; ++j) {
+        h[j] = fmaf(f[k][j], h[j], q[k][j]);
+        o[j] = k < live ? h[j] : 0.f;
+      }
+      if (k < there) at.store(row((char*)d.y, d.y_batch, d.y_row, k), yl, o);
     }
-    if (k < there) at.store(row((char*)d.y, d.y_batch, d.y_row, k), yl, o);
-  }
-  if (seg == 15 && u + 1 == a.units && d.h_last) at.store_state(d.h_last + bd, h);
+    if (seg == 15 && u + 1 == a.units && d.h_last) at.store_state(d.h_last + bd, h);
+  };
+  if (columns >= CG * V && len - first >= UNIT) unit(std::true_type{});  // (as for the maps)
+  else unit(std::false_type{});
 }
 
 // backward: h has to be known forwards and c backwards, so the segments are joined in both directions
@@ -472,93 +489,99 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(const ScanArgs a) {
   const unsigned rest = uniform(id / a.tiles), tile = id - rest * a.tiles, u = uniform(rest / d.B), b = rest - u * d.B;
   const unsigned v = a.units - 1 - u;  // from the start of time (where the maps were read last), and in the direction of the walk
   const long long first = (long long)u * UNIT;
-  const Place<TYPE, WIDE> at(cg, d.D - (int)tile * CG * V);
+  const int columns = d.D - (int)tile * CG * V;
   long long len = d.L;
   if (d.lengths) len = max(0LL, min((long long)d.lengths[b], len));
-  const int live = (int)min(max(len - first, 0LL), (long long)UNIT) - seg * TS, there = (int)min(d.L - first, (int64_t)UNIT) - seg * TS;
   const long long es = sizeof(typename Elem<TYPE>::T), bd = (long long)b * d.D + (long long)tile * CG * V;
   const auto row = [&](auto* p, int64_t batch, int64_t step, int k) { return p + (b * batch + (first + k) * step + (long long)tile * CG * V) * es; };
-  const auto lane = [&](int64_t step) { return (seg * TS * (unsigned)step + at.d0) * (unsigned)es; };
-  Raw<TYPE> x[TS], g[TS], dy[TS];
-  const unsigned xl = lane(d.x_row), gl = lane(d.gate_row), yl = lane(d.dy_row);
+  const auto unit = [&](auto whole) {
+    constexpr bool ALL = decltype(whole)::value;
+    const Place<TYPE, WIDE> at(cg, ALL ? CG * V : columns);
+    const int live = ALL ? UNIT : (int)min(max(len - first, 0LL), (long long)UNIT) - seg * TS, there = ALL ? UNIT : (int)min(d.L - first, (int64_t)UNIT) - seg * TS;
+    const auto lane = [&](int64_t step) { return (seg * TS * (unsigned)step + at.d0) * (unsigned)es; };
+    Raw<TYPE> x[TS], g[TS], dy[TS];
+    const unsigned xl = lane(d.x_row), gl = lane(d.gate_row), yl = lane(d.dy_row);
 #pragma unroll
-  for (int k = 0; k < TS; ++k) {
-    x[k].u = dy[k].u = fill_word<TYPE>(0u);
-    g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
-    if (k < live) {
-      x[k].u = at.load(row((const char*)d.x, d.x_batch, d.x_row, k), xl, 0u);
-      g[k].u = at.load(row((const char*)d.gate, d.gate_batch, d.gate_row, k), gl, Elem<TYPE>::PAD);
-      if (d.dy) dy[k].u = at.load(row((const char*)d.dy, d.dy_batch, d.dy_row, k), yl, 0u);
+    for (int k = 0; k < TS; ++k) {
+      x[k].u = dy[k].u = fill_word<TYPE>(0u);
+      g[k].u = fill_word<TYPE>(Elem<TYPE>::PAD);
+      if (k < live) {
+        x[k].u = at.load(row((const char*)d.x, d.x_batch, d.x_row, k), xl, 0u);
+        g[k].u = at.load(row((const char*)d.gate, d.gate_batch, d.gate_row, k), gl, Elem<TYPE>::PAD);
+        if (d.dy) dy[k].u = at.load(row((const char*)d.dy, d.dy_batch, d.dy_row, k), yl, 0u);
+      }
     }
-  }
-  float h[V], back[V];
-  at.load_state(d.states + u * BD + bd, h);
+    float h[V], back[V];
+    at.load_state(d.states + u * BD + bd, h);
 #pragma unroll
-  for (int j = 0; j < V; ++j) back[j] = 0.f;
-  if (a.units > 1) at.load_state(a.states + v * BD + bd, back);
-  else if (d.dh_last) at.load_state(d.dh_last + bd, back);
+    for (int j = 0; j < V; ++j) back[j] = 0.f;
+    if (a.units > 1) at.load_state(a.states + v * BD + bd, back);
+    else if (d.dh_last) at.load_state(d.dh_last + bd, back);
 
-  float f[TS][V], i[TS][V], P[V], Q[V], R[V], pf[V], qf[V], pb[V], rb[V];
+    float f[TS][V], i[TS][V], P[V], Q[V], R[V], pf[V], qf[V], pb[V], rb[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; R[j] = 0.f; }
+    for (int j = 0; j < V; ++j) { P[j] = 1.f; Q[j] = 0.f; R[j] = 0.f; }
 #pragma unroll
-  for (int k = 0; k < TS; ++k)
+    for (int k = 0; k < TS; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        gate_of<TYPE>(g[k].get(j), f[k][j], i[k][j]);
+        P[j] *= f[k][j];
+        Q[j] = fmaf(f[k][j], Q[j], i[k][j] * x[k].get(j));
+      }
+#pragma unroll
+    for (int k = TS - 1; k >= 0; --k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) R[j] = f[k][j] * (dy[k].get(j) + R[j]);
+    wave_join_both(P, Q, R, pf, qf, pb, rb);
+    if ((threadIdx.x & 48) == 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        wave_map[wave][cg][j] = make_float2(P[j], Q[j]);
+        wave_back[wave][cg][j] = R[j];
+      }
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; ++w)  // the state in front of this wave
+#pragma unroll
+      for (int j = 0; j < V; ++j) h[j] = fmaf(wave_map[w][cg][j].x, h[j], wave_map[w][cg][j].y);
+    for (int w = 3; w > wave; --w)  // and what the waves behind it hand on
+#pragma unroll
+      for (int j = 0; j < V; ++j) back[j] = fmaf(wave_map[w][cg][j].x, back[j], wave_back[w][cg][j]);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      gate_of<TYPE>(g[k].get(j), f[k][j], i[k][j]);
-      P[j] *= f[k][j];
-      Q[j] = fmaf(f[k][j], Q[j], i[k][j] * x[k].get(j));
+      h[j] = fmaf(pf[j], h[j], qf[j]);
+      back[j] = fmaf(pb[j], back[j], rb[j]);  // c_(t+1) of the segment's last step
     }
+    float hx[TS][V];  // h_(t-1) - x_t, forwards
 #pragma unroll
-  for (int k = TS - 1; k >= 0; --k)
+    for (int k = 0; k < TS; ++k)
 #pragma unroll
-    for (int j = 0; j < V; ++j) R[j] = f[k][j] * (dy[k].get(j) + R[j]);
-  wave_join_both(P, Q, R, pf, qf, pb, rb);
-  if ((threadIdx.x & 48) == 0) {
+      for (int j = 0; j < V; ++j) {
+        const float xv = x[k].get(j);
+        hx[k][j] = h[j] - xv;
+        h[j] = fmaf(f[k][j], h[j], i[k][j] * xv);
+      }
+    const unsigned xo = lane(d.dx_row), go = lane(d.dgate_row);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      wave_map[wave][cg][j] = make_float2(P[j], Q[j]);
-      wave_back[wave][cg][j] = R[j];
+    for (int k = TS - 1; k >= 0; --k) {
+      float ox[V], og[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float dh = dy[k].get(j) + back[j], di = dh * i[k][j];
+        ox[j] = k < live ? di : 0.f;
+        og[j] = k < live ? di * f[k][j] * hx[k][j] : 0.f;
+        back[j] = f[k][j] * dh;
+      }
+      if (k < there) {
+        if (d.dx) at.store(row((char*)d.dx, d.dx_batch, d.dx_row, k), xo, ox);
+        if (d.dgate) at.store(row((char*)d.dgate, d.dgate_batch, d.dgate_row, k), go, og);
+      }
     }
-  }
-  __syncthreads();
-  for (int w = 0; w < wave; ++w)  // the state in front of this wave
-#pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = fmaf(wave_map[w][cg][j].x, h[j], wave_map[w][cg][j].y);
-  for (int w = 3; w > wave; --w)  // and what the waves behind it hand on
-#pragma unroll
-    for (int j = 0; j < V; ++j) back[j] = fmaf(wave_map[w][cg][j].x, back[j], wave_back[w][cg][j]);
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    h[j] = fmaf(pf[j], h[j], qf[j]);
-    back[j] = fmaf(pb[j], back[j], rb[j]);  // c_(t+1) of the segment's last step
-  }
-  float hx[TS][V];  // h_(t-1) - x_t, forwards
-#pragma unroll
-  for (int k = 0; k < TS; ++k)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float xv = x[k].get(j);
-      hx[k][j] = h[j] - xv;
-      h[j] = fmaf(f[k][j], h[j], i[k][j] * xv);
-    }
-  const unsigned xo = lane(d.dx_row), go = lane(d.dgate_row);
-#pragma unroll
-  for (int k = TS - 1; k >= 0; --k) {
-    float ox[V], og[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float dh = dy[k].get(j) + back[j], di = dh * i[k][j];
-      ox[j] = k < live ? di : 0.f;
-      og[j] = k < live ? di * f[k][j] * hx[k][j] : 0.f;
-      back[j] = f[k][j] * dh;
-    }
-    if (k < there) {
-      if (d.dx) at.store(row((char*)d.dx, d.dx_batch, d.dx_row, k), xo, ox);
-      if (d.dgate) at.store(row((char*)d.dgate, d.dgate_batch, d.dgate_row, k), go, og);
-    }
-  }
-  if (seg == 0 && u == 0 && d.dh0) at.store_state(d.dh0 + bd, back);
+    if (seg == 0 && u == 0 && d.dh0) at.store_state(d.dh0 + bd, back);
+  };
+  if (columns >= CG * V && len - first >= UNIT) unit(std::true_type{});
+  else unit(std::false_type{});
 }
 
 inline int esize(int type) { return type == 0 ? 4 : 2; }
