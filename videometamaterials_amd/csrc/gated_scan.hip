@@ -177,9 +177,9 @@ __device__ __forceinline__ void wave_join(float* p, float* q, float* pe, float* 
 }
 
 // Consecutive workgroups go to different XCDs.  Where rows do not start on cache lines, each XCD gets a run of the work instead, so that tiles beside each
-// other share the lines at their borders in one L2: 4093 steps of 8 x 1000 channels in bf16 take 30 / 40 / 31 / 71 us for forward maps and application,
-// backward maps and application where the plain order takes 36 / 48 / 35 / 86; rows that do (1024 channels) are up to 6 % faster in the plain
-// order.  The grid is eight runs; numbers from `work` on are nobody's.
+// other share the lines at their borders in one L2: 4093 steps of 8 x 1000 channels in bf16 take 26 / 33 / 27 / 68 us for forward maps and application,
+// backward maps and application where the plain order takes 33 / 47 / 33 / 86; rows that do (65536 x 1024) 56 / 69 us in the plain order and
+// 60 / 70 in runs.  The grid is eight runs; numbers from `work` on are nobody's.
 __device__ __forceinline__ unsigned number(const ScanArgs& a, unsigned work) {
   return a.runs ? (blockIdx.x & 7) * ((work + 7) / 8) + (blockIdx.x >> 3) : blockIdx.x;
 }
@@ -205,7 +205,8 @@ __device__ __forceinline__ void wave_join_both(float* p, float* q, float* r, flo
 }
 
 // ---- step 1.  A workgroup makes the maps of a group: a wave a unit, a lane 4 channels and a quarter of its steps, four at a time with the next ones on
-// their way (eight at a time need more registers than 16 waves have: 75 us where four take 64 for 65536 steps of 1024 channels in bf16).  Forward from x and gate, BACK from dy and gate.
+// their way (eight at a time need more registers than 16 waves have, and took a sixth longer).
+// Forward from x and gate, BACK from dy and gate.
 template <int TYPE, bool WIDE, bool BACK>
 __global__ __launch_bounds__(1024) void scan_map_kernel(const ScanArgs a) {
   constexpr int STEPS = UNIT / 4, BATCH = 4, BATCHES = STEPS / BATCH;
@@ -475,7 +476,8 @@ __global__ __launch_bounds__(256, 5) void scan_fwd_kernel(const ScanArgs a) {
   else unit(std::false_type{});
 }
 
-// backward: h has to be known forwards and c backwards, so the segments are joined in both directions
+// backward: h has to be known forwards and c backwards, so the segments are joined in both directions.  Three workgroups a CU: for four, 28 registers would
+// have to go to scratch (8 x 4093 x 1000 bf16: 105 us, here 68).
 template <int TYPE, bool WIDE>
 __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(const ScanArgs a) {
   constexpr int TS = UNIT / 16;
