@@ -779,7 +779,9 @@ int vmm_conv_igemm_fp16_batched(const vmm_conv_desc* descs, int32_t n, vmm_strea
  *   dh_t = dy_t + f_(t+1) dh_(t+1),  dx = dh (1 - f),  dgate = dh (h_(t-1) - x) f (1 - f),  dh0 = f_1 dh_1;  zero behind the length.
  * dy, dh_last (NULL = zero), dx, dgate, dh0 (each may be NULL) as the tensors they belong to.
  * workspace: vmm_gated_scan_workspace bytes, 16-byte aligned, contents irrelevant, for one call at a time; NULL where that is 0.  The result does
- * not depend on how workgroups fall: the same bits every time. */
+ * not depend on how workgroups fall: the same bits every time.
+ * Refused (-1, by the queries too): L or B D of 2^31 and more, row strides of 2^23 and more, and what would take 2^32 threads a launch:
+ * B ceil(D / 64) ceil(L / 64) near 2^24, and beyond 64 steps B ceil(D / 64) ceil(L / 1024) near 2^22. */
 int64_t vmm_gated_scan_states(const vmm_gated_scan_desc* d);
 int64_t vmm_gated_scan_workspace(const vmm_gated_scan_desc* d, int32_t backward);
 int vmm_gated_scan(const vmm_gated_scan_desc* d, vmm_stream_t stream);
@@ -791,7 +793,8 @@ int vmm_gated_scan_bwd(const vmm_gated_scan_desc* d, vmm_stream_t stream);
  * Training: the forward leaves g = x Wg^T + bg and u = x Wu^T + bu in fp32, [M][F] each (g_pre, u_pre; both NULL: not kept).  Backward from dh:
  *   du = dh act(g), dg = dh u act'(g) (rounded to `type`: they are the operands of the products below),
  *   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dbg, dbu = column sums.   dx, (dWg, dWu), (dbg, dbu): each pair may be NULL; they are WRITTEN.
- * workspace: vmm_gated_ff_workspace bytes, 16-byte aligned, contents irrelevant, for one call at a time; NULL where that is 0. */
+ * workspace: vmm_gated_ff_workspace bytes, 16-byte aligned, contents irrelevant, for one call at a time; NULL where that is 0.
+ * Refused (-1, by the query too): M of 2^31 and more, K, F, ldx, ldh, lddx of 2^22 and more, and 2^23 tiles of 256 x 256 in a product. */
 int64_t vmm_gated_ff_workspace(const vmm_gated_ff_desc* d, int32_t backward);
 int vmm_gated_ff(const vmm_gated_ff_desc* d, vmm_stream_t stream);
 int vmm_gated_ff_bwd(const vmm_gated_ff_desc* d, vmm_stream_t stream);

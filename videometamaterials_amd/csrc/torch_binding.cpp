@@ -134,7 +134,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &gate = saved[1], &states = saved[3];
+    const Tensor &x = saved[0], &gate = saved[1], &lengths = saved[2], &states = saved[3];
     if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     Tensor dx, dgate, dh0;
     {
@@ -144,7 +144,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
       if (ctx->needs_input_grad(0)) dx = same(x.sizes(), x);
       if (ctx->needs_input_grad(1)) dgate = same(x.sizes(), x);
       if (ctx->saved_data["state"].toBool() && ctx->needs_input_grad(2)) dh0 = fp32({x.size(0), x.size(2)}, x);
-      vmm_gated_scan_desc d = scan_desc(x, gate, saved[3 - 1].defined() ? Maybe(saved[2]) : Maybe());
+      vmm_gated_scan_desc d = scan_desc(x, gate, lengths.defined() ? Maybe(lengths) : Maybe());
       place(dy, d.dy, d.dy_batch, d.dy_row);
       place(dx, d.dx, d.dx_batch, d.dx_row);
       place(dgate, d.dgate, d.dgate_batch, d.dgate_row);
