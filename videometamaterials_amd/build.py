@@ -42,9 +42,6 @@ SINGLE_PASS_SOURCES = {"temporal_block_bwd.hip", "linattn_block_bwd.hip", "qkv_b
 #   and then (the host pass of hipcc does not know the feature and says so; harmless)
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=on", "-munsafe-fp-atomics", "-fno-slp-vectorize", *NO_PACKED_FP32]
-# temporal_block.hip holds no packed fp32 instruction either way (its assembly has none without the flag), and is compiled as it always was: under the flag it
-# is scheduled differently, and the C = 128 block without tokens then gives other results from run to run (1.6e-2 off; as it is: 1.4e-5, the same bits)
-WITHOUT_THE_FLAG = {"temporal_block.hip"}
 if EXPERIMENTS:
     FLAGS.append("-DVMM_EXPERIMENTS=1")
 
@@ -66,11 +63,6 @@ def _flags_changed(cmd) -> bool:
         return True
 
 
-def _flags(source: str) -> list:
-    plain = [f for f in FLAGS if f not in NO_PACKED_FP32]
-    return plain if os.path.basename(source) in WITHOUT_THE_FLAG else FLAGS
-
-
 def build(force: bool = False, verbose: bool = True) -> str:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     srcs = [s for s in sorted(glob.glob(os.path.join(CSRC, "*.hip"))) if EXPERIMENTS or os.path.basename(s) not in EXPERIMENT_SOURCES]
@@ -80,20 +72,20 @@ def build(force: bool = False, verbose: bool = True) -> str:
     for s in srcs:
         o = os.path.join(OBJDIR, os.path.basename(s)[:-4] + ".o")
         objs.append(o)
-        cmd = [hipcc, *_flags(s), "-c", s, "-o", o]
+        cmd = [hipcc, *FLAGS, "-c", s, "-o", o]
         if force or _stale(o, [s] + hdrs) or _flags_changed(cmd):
             jobs.append(cmd)
         if EXPERIMENTS and os.path.basename(s) in SPLIT_F16_SOURCES:  # (experiments library only: measured, worth 0-4 % of a block, not used by any plan -- LABNOTES 11.2)
             o3 = o[:-2] + "_f3.o"
             objs.append(o3)
-            cmd = [hipcc, *_flags(s), "-DVMM_SPLIT_F16=1", "-c", s, "-o", o3]
+            cmd = [hipcc, *FLAGS, "-DVMM_SPLIT_F16=1", "-c", s, "-o", o3]
             if force or _stale(o3, [s] + hdrs) or _flags_changed(cmd):
                 jobs.append(cmd)
         if os.path.basename(s) in SINGLE_PASS_SOURCES or os.path.basename(s) in FP16_FORWARD_SOURCES:
             for tag, mode in (SINGLE_PASS_MODES if os.path.basename(s) in SINGLE_PASS_SOURCES else SINGLE_PASS_MODES[1:]):
                 o2 = o[:-2] + tag + ".o"
                 objs.append(o2)
-                cmd = [hipcc, *_flags(s), f"-DVMM_SINGLE_PASS={mode}", "-c", s, "-o", o2]
+                cmd = [hipcc, *FLAGS, f"-DVMM_SINGLE_PASS={mode}", "-c", s, "-o", o2]
                 if force or _stale(o2, [s] + hdrs) or _flags_changed(cmd):
                     jobs.append(cmd)
     if jobs:

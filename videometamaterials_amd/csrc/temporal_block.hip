@@ -935,13 +935,19 @@ __global__ __launch_bounds__(512, 2) void temporal_block2_kernel(const TBArgs a)
         uint4 qh[2], ql[2];
         split8(qt, 0, qh[0], ql[0]);
         split8(qt, 8, qh[1], ql[1]);
+        // The token scores come first.  Behind the frame scores, their branch stood between a product and its first reader, and the compiler (ROCm 7.2) counts
+        // the wait states of a result along the way through a branch and not along the one around it: without tokens, the softmax read the scores 5
+        // wait states after the last product where the hardware needs 11 (and does not wait by itself).
         f32x16 st = zero16(), sk = zero16();
+        if (ntok) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) sk = mfma3<ONE>(eks_l[(s * 2) * 32], eks_l[(s * 2 + 1) * 32], qh[s], ql[s], sk);
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           uint4 kh, kl;
           split8(kt, s * 8, kh, kl);
           st = mfma3<ONE>(kh, kl, qh[s], ql[s], st);
-          if (ntok) sk = mfma3<ONE>(eks_l[(s * 2) * 32], eks_l[(s * 2 + 1) * 32], qh[s], ql[s], sk);
         }
         // logits of this lane's query: 8 (16) frame keys and 8 tokens per lane half, relative-position bias from LDS
         float bz[NK];
