@@ -49,3 +49,60 @@ def test_ff_same_bits_between_other_calls_and_how_far_from_64(gpu, dtype, M, K, 
     for k, (got, w) in enumerate(zip(want, exact)):
         off, alone = float((got.double() - w).norm()), float((w.to(dtype).double() - w).norm())
         assert off < (1.05 if k == 0 else 1.05 * math.sqrt(2)) * alone, k
+
+
+def scan_reference(x, gate, h0, dy, dlast):
+    """y, last, dx, dgate, dh0 of the recurrence in 64 bits, and beside each the same sums over absolute values, by which its error is measured: an operator that keeps
+    every factor to a few roundings of fp32 stays within those roundings of them, however small a result is."""
+    x, gate, h0, dy, dlast = (v.detach().double().cpu() for v in (x, gate, h0, dy, dlast))
+    L = x.shape[1]
+    f, i = torch.sigmoid(gate), torch.sigmoid(-gate)
+
+    def run(x, h0, dy, dlast, less):
+        h, before, y = h0, [], []
+        for t in range(L):
+            before.append(h)
+            h = f[:, t] * h + i[:, t] * x[:, t]
+            y.append(h)
+        c, dx, dg = dlast, [None] * L, [None] * L
+        for t in reversed(range(L)):
+            dh = dy[:, t] + c
+            dx[t], dg[t] = dh * i[:, t], dh * less(before[t], x[:, t]) * f[:, t] * i[:, t]
+            c = f[:, t] * dh
+        return torch.stack(y, 1), h, torch.stack(dx, 1), torch.stack(dg, 1), c
+    return zip(run(x, h0, dy, dlast, lambda a, b: a - b), run(x.abs(), h0.abs(), dy.abs(), dlast.abs(), lambda a, b: a + b))
+
+
+def scan_all(x, gate, h0, dy, dlast):
+    from videometamaterials_amd import gated_linear_scan
+    leaves = [v.detach().requires_grad_() for v in (x, gate, h0)]
+    y, last = gated_linear_scan(*leaves)
+    return (y.detach(), last.detach(), *torch.autograd.grad((y, last), leaves, (dy, dlast)))
+
+
+def within(got, want, bound, what):
+    off = (got.detach().double().cpu() - want).abs() - bound
+    at = int(off.argmax())
+    assert float(off.max()) <= 0, f"{what}: {float(got.flatten()[at])} for {float(want.flatten()[at])}, {float(bound.flatten()[at])} allowed, at {at}"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("L", [1, 40, 300])
+@pytest.mark.parametrize("x_size", [1.0, 0.0])
+def test_scan_closed_gates(gpu, dtype, L, x_size):
+    """Forget gates of e^-8 to e^-19 (and open ones beside them): dgate, dh0 and states that come through a closed gate are proportional to it, so it has to be
+    right relative to itself.  A gate is off by (|g| + 4) U of itself; a state passes at most some 20 gates that are not closed before it is gone."""
+    n = normal(gpu, 17)
+    x, h0, dy, dlast = n(2, L, 24, k=x_size, dtype=dtype), n(2, 24), n(2, L, 24, dtype=dtype), n(2, 24)
+    gate = torch.linspace(-19.0, -8.0, 24, device=gpu).expand(2, L, 24) + n(2, L, 24, k=0.3)
+    gate[:, ::7, ::5] = 2.0
+    gate = gate.to(dtype)
+    rel = 8 * (float(gate.abs().max()) + 4) * U
+    # What ends below a type's smallest normal number is a multiple of its smallest number (2^-24, 2^-133, 2^-149) and loses half of that, whatever its size: y, dx and
+    # dgate once in their type, a state of fp32 at every gate it passes -- 1 / (1 - f) = 8.4 of them are alive behind open gates of f = sigmoid(2), twice that
+    # for maps that were joined before they were applied.
+    sub = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150}[dtype]
+    small = 17 * 2.0 ** -150
+    for what, got, (want, size) in zip(("y", "last", "dx", "dgate", "dh0"), scan_all(x, gate, h0, dy, dlast), scan_reference(x, gate, h0, dy, dlast)):
+        held = (half_step(dtype) * want.abs() + sub) if got.dtype == dtype else 0.0
+        within(got, want, held + (rel * size + small) * (1 + half_step(dtype)), what)

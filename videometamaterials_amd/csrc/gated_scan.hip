@@ -120,12 +120,11 @@ struct Place {
 // a value that is the same in every lane, in a scalar register
 __device__ __forceinline__ unsigned uniform(unsigned v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// f = sigmoid(g) and i = 1 - f = sigmoid(-g).  These kernels are bound by their instructions as much as by memory, and the gate is a third of them.
-// 16 bits: i = 1 / (1 + e^g), f = 1 - i, whatever e^g is, zero and infinite too.  The gates that are multiplied with themselves over a whole memory, f near
-// one, have one rounding -- the error of a reciprocal would add up there; f near zero is off by a rounding of one, as its products with states and
-// inputs of one's size are anyway.
-// fp32: each accurate in itself.  e = exp(-|g|), the smaller of the two is e / (1 + e), the larger 1 minus that; exp is corrected for what rounding
-// p = -|g| log2(e) has lost, up to |g| 2^-25 of e.  NaN passes in both.
+// f = sigmoid(g) and i = 1 - f = sigmoid(-g), each accurate in itself: dgate and dh0 are proportional to f, and f is multiplied with itself over a whole memory.  The smaller
+// of the two is e / (1 + e) with e = e^-|g|, the larger 1 minus that, which has one rounding (the error of a reciprocal would add up over a memory).
+// 16 bits: i = 1 / (1 + e^g) serves either way, zero and infinite e^g too; f = 1 - i where the gate is open and e^g i where it is closed, where 1 - i has lost it
+// (by a sixth at g = -15, all of it from -17 on).
+// fp32: exp is corrected for what rounding p = -|g| log2(e) has lost, up to |g| 2^-25 of e.  NaN passes in both.
 template <int TYPE>
 __device__ __forceinline__ void gate_of(float g, float& f, float& i) {
   if constexpr (TYPE == 0) {
@@ -140,8 +139,9 @@ __device__ __forceinline__ void gate_of(float g, float& f, float& i) {
     f = g < 0.f ? small : large;
     i = g < 0.f ? large : small;
   } else {
-    i = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * 1.44269502162933349609375f));
-    f = 1.0f - i;
+    const float e = __builtin_amdgcn_exp2f(g * 1.44269502162933349609375f);
+    i = __builtin_amdgcn_rcpf(1.0f + e);
+    f = g < 0.f ? e * i : 1.0f - i;
   }
 }
 
