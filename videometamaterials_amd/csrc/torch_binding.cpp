@@ -27,6 +27,8 @@ struct Entries {
 
 // becomes videometamaterials_amd._native.NativeError
 struct NativeFault : std::runtime_error { using std::runtime_error::runtime_error; };
+// becomes NotImplementedError
+struct Unsupported : std::runtime_error { using std::runtime_error::runtime_error; };
 
 template <typename E, typename... Args>
 [[noreturn]] void fail(const Args&... args) { throw E(c10::str(args...)); }
@@ -46,6 +48,14 @@ int type_of(const Tensor& t) {
 
 void need_gpu(const Tensor& t, const char* what) {
   if (!t.is_cuda()) fail<NativeFault>(what, ": tensors must live on the GPU (there is no CPU path)");
+}
+
+// What is computed through raw pointers has no derivative in forward mode: a tangent would vanish without a word.
+void need_plain(const Tensor& t, const char* what) {
+  if (t.unsafeGetTensorImpl()->_fw_grad(0, t).defined()) fail<Unsupported>(what, ": no forward-mode derivative");
+}
+void need_plain(const Maybe& t, const char* what) {
+  if (t) need_plain(*t, what);
 }
 
 vmm_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
@@ -159,6 +169,9 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
 };
 
 std::tuple<Tensor, Tensor> gated_linear_scan(Tensor x, Tensor gate, Maybe h0, Maybe lengths) {
+  need_plain(x, SCAN);
+  need_plain(gate, SCAN);
+  need_plain(h0, SCAN);
   if (x.dim() != 3 || gate.sizes() != x.sizes()) fail<py::value_error>(SCAN, ": x and gate must be (B, L, D) and alike, got ", shape(x), " and ", shape(gate));
   if (type_of(x) < 0 || gate.scalar_type() != x.scalar_type())
     fail<py::type_error>(SCAN, ": x and gate must be float32, bfloat16 or float16 alike, got ", x.scalar_type(), " and ", gate.scalar_type());
@@ -269,6 +282,7 @@ Tensor gated_feed_forward(const Tensor& x, const Tensor& w_gate, const Tensor& w
   const Tensor* every[5] = {&x, &w_gate, &w_up, b_gate ? &*b_gate : nullptr, b_up ? &*b_up : nullptr};
   const int n = b_gate ? 5 : 3;
   bool grad = false;
+  for (int i = 0; i < n; ++i) need_plain(*every[i], FF);
   for (int i = 3; i < n; ++i)
     if (every[i]->sizes() != at::IntArrayRef({F})) fail<py::value_error>(FF, ": biases must be (", F, ",), got ", shape(*every[i]));
   for (int i = 0; i < n; ++i) {
@@ -313,6 +327,7 @@ Listed listed(const py::object& sequence, const char* what) {
 }
 
 void check_grads(const std::vector<const Tensor*>& grads, const char* what) {
+  for (const Tensor* g : grads) need_plain(*g, what);
   for (const Tensor* g : grads)
     if (type_of(*g) < 0) fail<py::type_error>(what, ": float32, bfloat16 or float16 tensors, got ", g->scalar_type());
   for (const Tensor* g : grads)
@@ -404,9 +419,11 @@ Maybe clipped_adam(const py::object& params, const py::object& exp_avgs, const p
   std::vector<vmm_clip_adam_job> jobs(g.size());
   for (size_t k = 0; k < g.size(); ++k) {
     const Tensor* own[3] = {p.tensors[at_[k]], m.tensors[at_[k]], v.tensors[at_[k]]};
-    for (const Tensor* t : own)
+    for (const Tensor* t : own) {
+      need_plain(*t, what);
       if (t->device() != g[0]->device() || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->numel() != g[k]->numel())
         fail<py::value_error>(what, ": parameters and moments must be contiguous float32 tensors of one size, on the gradients' device");
+    }
     jobs[k] = {ptr<float>(*own[0]), g[k]->data_ptr(), ptr<float>(*own[1]), ptr<float>(*own[2]), g[k]->numel(), type_of(*g[k]), 0};
   }
   const c10::DeviceGuard guard(g[0]->device());
@@ -433,6 +450,8 @@ PYBIND11_MODULE(_sequence, m) {
       if (p) std::rethrow_exception(p);
     } catch (const NativeFault& e) {
       py::set_error(py::module_::import("videometamaterials_amd._native").attr("NativeError"), e.what());
+    } catch (const Unsupported& e) {
+      py::set_error(PyExc_NotImplementedError, e.what());
     }
   });
   m.attr("entries") = [] {
