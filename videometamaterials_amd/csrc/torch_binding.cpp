@@ -6,7 +6,10 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include "../../include/vmm_kernels.h"
 
@@ -50,12 +53,26 @@ void need_gpu(const Tensor& t, const char* what) {
   if (!t.is_cuda()) fail<NativeFault>(what, ": tensors must live on the GPU (there is no CPU path)");
 }
 
-// What is computed through raw pointers has no derivative in forward mode: a tangent would vanish without a word.
+// What is computed through raw pointers has no derivative in forward mode (a tangent would vanish without a word), and no tensor can stand in for another
+// (subclasses, the wrappers of torch.func, lazily negated views).
 void need_plain(const Tensor& t, const char* what) {
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet stand_ins{DispatchKey::Python,      DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper, DispatchKey::Functionalize,
+                                          DispatchKey::ZeroTensor, DispatchKey::Negative};
   if (t.unsafeGetTensorImpl()->_fw_grad(0, t).defined()) fail<Unsupported>(what, ": no forward-mode derivative");
+  if (t.unsafeGetTensorImpl()->key_set().has_any(stand_ins)) fail<Unsupported>(what, ": plain tensors only (no subclass, torch.func transform or lazy negation)");
 }
 void need_plain(const Maybe& t, const char* what) {
   if (t) need_plain(*t, what);
+}
+
+// Nothing that records operations instead of running them sees these: a trace would hold empty buffers that nobody fills.
+void need_eager(const char* what) {
+  using c10::impl::TorchDispatchModeTLS;
+  using c10::impl::TorchDispatchModeKey;
+  if (torch::jit::tracer::isTracing() || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE) ||
+      TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FUNCTIONAL) || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch))
+    fail<Unsupported>(what, ": cannot be traced (torch.jit.trace, make_fx, torch.export, fake tensors)");
 }
 
 vmm_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
@@ -169,6 +186,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
 };
 
 std::tuple<Tensor, Tensor> gated_linear_scan(Tensor x, Tensor gate, Maybe h0, Maybe lengths) {
+  need_eager(SCAN);
   need_plain(x, SCAN);
   need_plain(gate, SCAN);
   need_plain(h0, SCAN);
@@ -275,6 +293,7 @@ struct GatedFF : torch::autograd::Function<GatedFF> {
 };
 
 Tensor gated_feed_forward(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const Maybe& b_gate, const Maybe& b_up, int64_t act) {
+  need_eager(FF);
   if (x.dim() < 1 || w_gate.dim() != 2 || w_up.sizes() != w_gate.sizes() || x.size(-1) != w_gate.size(1) || w_gate.numel() == 0)
     fail<py::value_error>(FF, ": x (..., K) and weights (F, K) do not fit: ", shape(x), ", ", shape(w_gate), ", ", shape(w_up));
   if (b_gate.has_value() != b_up.has_value()) fail<py::value_error>(FF, ": both biases or none");
@@ -327,6 +346,7 @@ Listed listed(const py::object& sequence, const char* what) {
 }
 
 void check_grads(const std::vector<const Tensor*>& grads, const char* what) {
+  need_eager(what);
   for (const Tensor* g : grads) need_plain(*g, what);
   for (const Tensor* g : grads)
     if (type_of(*g) < 0) fail<py::type_error>(what, ": float32, bfloat16 or float16 tensors, got ", g->scalar_type());

@@ -1,8 +1,9 @@
 """Operators of sequence encoders: the gated linear recurrence (csrc/gated_scan.hip) and the gated feed-forward product (csrc/gated_ff.hip), each with its
 gradients.  They stand beside the GRU of ``cond_att_GRU`` (vddp.py:546-549): a recurrence that is scanned in parallel over time, and the mixing of
 channels behind it; ``Unet3D(cond_att_scan=True)`` builds its load-history encoder from them.
-Checks, workspaces, launches and the autograd nodes are compiled (csrc/torch_binding.cpp).  Gradients are those of the backward pass; forward-mode derivatives are
-refused (NotImplementedError).
+Checks, workspaces, launches and the autograd nodes are compiled (csrc/torch_binding.cpp).  Gradients are those of the backward pass; forward-mode derivatives,
+the transforms of torch.func, tracing (torch.jit.trace, make_fx, torch.export) and tensors that stand in for others are refused (NotImplementedError); torch.compile
+breaks its graph around a call.
 """
 from __future__ import annotations
 
