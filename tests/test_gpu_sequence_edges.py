@@ -106,3 +106,21 @@ def test_scan_closed_gates(gpu, dtype, L, x_size):
     for what, got, (want, size) in zip(("y", "last", "dx", "dgate", "dh0"), scan_all(x, gate, h0, dy, dlast), scan_reference(x, gate, h0, dy, dlast)):
         held = (half_step(dtype) * want.abs() + sub) if got.dtype == dtype else 0.0
         within(got, want, held + (rel * size + small) * (1 + half_step(dtype)), what)
+
+
+@pytest.mark.parametrize("kind", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.uint16, torch.uint32, torch.uint64])
+def test_scan_lengths_of_every_integer_type(gpu, kind):
+    """Sequences longer than the type can say, values outside 0 .. L."""
+    from videometamaterials_amd import gated_linear_scan
+    n = normal(gpu, 1)
+    x, gate = n(4, 300, 8), n(4, 300, 8)
+    info = torch.iinfo(kind)
+    values = [info.min, info.max, 0, 77]
+    y, last = gated_linear_scan(x, gate, lengths=torch.tensor(values, dtype=kind).to(gpu))
+    want, _ = gated_linear_scan(x, gate)
+    for b, v in enumerate(values):
+        v = min(max(v, 0), 300)
+        assert torch.equal(y[b, :v], want[b, :v]) and not y[b, v:].any()
+        assert torch.equal(last[b], gated_linear_scan(x[b:b + 1, :v], gate[b:b + 1, :v])[1][0])
+    with pytest.raises(ValueError):
+        gated_linear_scan(x, gate, lengths=torch.ones(4, device=gpu, dtype=torch.bool))

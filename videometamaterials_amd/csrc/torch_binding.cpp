@@ -203,7 +203,11 @@ std::tuple<Tensor, Tensor> gated_linear_scan(Tensor x, Tensor gate, Maybe h0, Ma
     fail<py::value_error>(SCAN, ": all tensors must be on ", x.device().str());
   if (std::max({B, D}) >= (1LL << 31)) fail<py::value_error>(SCAN, ": a size is out of range");
   if (h0) h0 = h0->to(at::kFloat).contiguous();
-  if (lengths) lengths = lengths->scalar_type() == at::kInt ? lengths->contiguous() : lengths->clamp(0, L).to(at::kInt);
+  if (lengths && lengths->scalar_type() != at::kInt) {  // (in 64 bits before L is compared with: it need not fit a narrow type; and from 2^63 on they are beyond any L)
+    const Tensor wide = lengths->to(at::kLong);
+    lengths = (lengths->scalar_type() == at::kUInt64 ? at::where(wide.lt(0), L, wide) : wide).clamp(0, L).to(at::kInt);
+  }
+  if (lengths) lengths = lengths->contiguous();
   x = rows_of(x);
   gate = rows_of(gate);
   if (c10::GradMode::is_enabled() && (x.requires_grad() || gate.requires_grad() || (h0 && h0->requires_grad()))) {
