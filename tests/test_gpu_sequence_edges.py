@@ -121,6 +121,9 @@ def test_scan_lengths_of_every_integer_type(gpu, kind):
     for b, v in enumerate(values):
         v = min(max(v, 0), 300)
         assert torch.equal(y[b, :v], want[b, :v]) and not y[b, v:].any()
-        assert torch.equal(last[b], gated_linear_scan(x[b:b + 1, :v], gate[b:b + 1, :v])[1][0])
+        # (The last state of a padded sequence comes through maps that are joined in an order of L, not of v: another order of the same sums.  A step rounds three
+        # times; a state is a mean of inputs that forgets by f <= sigmoid(4.5) a step, 1 / (1 - f) < 92 steps in all; twice, for the two orders.)
+        alone = gated_linear_scan(x[b:b + 1, :v], gate[b:b + 1, :v])[1][0]
+        assert float(gate.max()) < 4.5 and float((last[b] - alone).abs().max()) <= 2 * 3 * 92 * U * float(x.abs().max())
     with pytest.raises(ValueError):
         gated_linear_scan(x, gate, lengths=torch.ones(4, device=gpu, dtype=torch.bool))
