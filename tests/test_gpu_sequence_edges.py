@@ -127,3 +127,27 @@ def test_scan_lengths_of_every_integer_type(gpu, kind):
         assert float(gate.max()) < 4.5 and float((last[b] - alone).abs().max()) <= 2 * 3 * 92 * U * float(x.abs().max())
     with pytest.raises(ValueError):
         gated_linear_scan(x, gate, lengths=torch.ones(4, device=gpu, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_of_dimensions_of_one(gpu, dtype):
+    """One token, one row, one channel: the stride of such a dimension says nothing, and may be any number in a tensor that counts as contiguous."""
+    from videometamaterials_amd import gated_feed_forward
+    n = normal(gpu, 3)
+    far = (1 << 40) + 3
+
+    def odd(t):
+        return torch.as_strided(t, t.shape, [far if size == 1 else stride for size, stride in zip(t.shape, t.stride())])
+    for B, L, D in ((3, 1, 64), (1, 1, 5), (1, 90, 20), (2, 90, 1), (1, 1, 1)):
+        x, gate, dy = (n(B, L, D, dtype=dtype) for _ in range(3))
+        h0, dlast = n(B, D), n(B, D)
+        got, want = scan_all(odd(x), odd(gate), odd(h0), odd(dy), odd(dlast)), scan_all(x, gate, h0, dy, dlast)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), (B, L, D)
+    for M, K, F in ((1, 64, 24), (1, 1, 1), (5, 1, 3), (5, 8, 1), (1, 9, 7)):
+        x, w, v, dh = n(M, K, dtype=dtype), n(F, K, dtype=dtype), n(F, K, dtype=dtype), n(M, F, dtype=dtype)
+        out = []
+        for change in (odd, lambda t: t):
+            leaves = [change(t).requires_grad_() for t in (x, w, v)]
+            h = gated_feed_forward(*leaves)
+            out.append((h, *torch.autograd.grad(h, leaves, change(dh))))
+        assert all(torch.equal(a, b) for a, b in zip(*out)), (M, K, F)

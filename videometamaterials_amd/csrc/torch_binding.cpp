@@ -79,10 +79,12 @@ vmm_stream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t
 
 std::string shape(const Tensor& t) { return c10::str(t.sizes()); }
 
-// `t` with neighbouring values in its last dimension and rows less than 2^22 values apart, as the kernels' 32-bit offsets need them (else a copy)
+// `t` with neighbouring values in its last dimension and rows less than 2^22 values apart, as the kernels' 32-bit offsets need them (else a copy).  The stride of
+// a dimension of one says nothing and may be anything, in a contiguous tensor too: it is neither looked at nor handed on.
 Tensor rows_of(const Tensor& t) {
-  return (t.stride(-1) == 1 || (t.size(-1) == 1 && t.is_contiguous())) && t.stride(-2) < (1 << 22) ? t : t.contiguous();
+  return (t.stride(-1) == 1 || t.size(-1) <= 1) && (t.stride(-2) < (1 << 22) || t.size(-2) <= 1) ? t : t.contiguous();
 }
+int64_t row_stride(const Tensor& t) { return t.size(-2) > 1 ? t.stride(-2) : t.size(-1); }
 
 template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
@@ -119,8 +121,8 @@ template <typename P>
 void place(const Tensor& t, P& p, int64_t& batch, int64_t& row) {
   if (!t.defined()) return;
   p = t.data_ptr();
-  batch = t.stride(0);
-  row = t.stride(1);
+  batch = t.size(0) > 1 ? t.stride(0) : 0;
+  row = row_stride(t);
 }
 
 vmm_gated_scan_desc scan_desc(const Tensor& x, const Tensor& gate, const Maybe& lengths) {
@@ -225,7 +227,7 @@ const char* const FF = "gated_feed_forward";
 vmm_gated_ff_desc ff_desc(const Tensor& x, const Tensor& wg, const Tensor& wu, int64_t act) {
   vmm_gated_ff_desc d = {};
   d.x = x.data_ptr();
-  d.ldx = x.stride(0);
+  d.ldx = row_stride(x);
   d.w_gate = wg.data_ptr();
   d.w_up = wu.data_ptr();
   d.M = x.size(0);
@@ -282,9 +284,9 @@ struct GatedFF : torch::autograd::Function<GatedFF> {
       d.g_pre = ptr<float>(pre);
       d.u_pre = d.g_pre + x.size(0) * wg.size(0);
       d.dh = dh.data_ptr();
-      d.lddh = dh.stride(0);
+      d.lddh = row_stride(dh);
       d.dx = ptr<void>(dx);
-      d.lddx = dx.defined() ? dx.stride(0) : 0;
+      d.lddx = dx.defined() ? row_stride(dx) : 0;
       d.dw_gate = ptr<void>(dwg);
       d.dw_up = ptr<void>(dwu);
       d.db_gate = ptr<void>(dbg);
