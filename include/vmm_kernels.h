@@ -769,7 +769,10 @@ int vmm_conv_igemm_fp16(const vmm_conv_desc* d, vmm_stream_t stream);
 int vmm_conv_igemm_fp16_batched(const vmm_conv_desc* descs, int32_t n, vmm_stream_t stream);
 
 /* ==== operators of sequence encoders and of their training (argument structs: vmm_sequence.h).  `type` of a buffer: 0 fp32, 1 bf16, 2 IEEE half;
- * strides count values of that type. ==== */
+ * strides count values of that type.
+ * The _workspace queries are asked with the very descriptor of the call, all of its pointers and strides set but the workspace's: which buffers are there, how they
+ * are aligned and how far apart rows are decides what has to be laid out or kept.  workspace_bytes is the size of the buffer that was provided; a call that
+ * needs more is refused (-1) and launches nothing. ==== */
 
 /* ---- gated linear recurrence over time, beside vmm_gru_recurrent: no product inside the loop, so the time axis is scanned in parallel.
  *   f = sigmoid(gate),  h_t = f_t h_(t-1) + (1 - f_t) x_t  for t < lengths[b],  y_t = h_t;   y = 0 and the state stands still behind the length.

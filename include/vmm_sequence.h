@@ -12,7 +12,7 @@ typedef struct vmm_gated_scan_desc {
   void* dx; int64_t dx_batch, dx_row;
   void* dgate; int64_t dgate_batch, dgate_row;
   const float* dh_last; float* dh0;
-  void* workspace;
+  void* workspace; int64_t workspace_bytes;
   int64_t L;
   int32_t B, D, type;
 } vmm_gated_scan_desc;
@@ -25,7 +25,7 @@ typedef struct vmm_gated_ff_desc {
   const void* dh; int64_t lddh;
   void* dx; int64_t lddx;
   void* dw_gate; void* dw_up; void* db_gate; void* db_up;
-  void* workspace;
+  void* workspace; int64_t workspace_bytes;
   int64_t M;
   int32_t K, F, type, act;
 } vmm_gated_ff_desc;

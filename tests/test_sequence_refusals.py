@@ -1,4 +1,6 @@
 """Calls that the sequence operators refuse before they look for a GPU."""
+import ctypes as C
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
@@ -63,3 +65,29 @@ def test_tensors_that_stand_in_for_others():
     assert isinstance(torch.nn.Parameter(x), torch.Tensor)
     with pytest.raises(Exception, match="GPU"):  # a parameter is a plain tensor
         gated_feed_forward(x, torch.nn.Parameter(w), w)
+
+
+def test_a_workspace_that_is_too_small_is_refused():
+    """Sizes depend on more than sizes: alignment, strides, which buffers are there.  A query without them gives less than the call needs; the call says so."""
+    from videometamaterials_amd import _native as N
+    lib = N.lib()
+    a = [(k + 1) << 24 for k in range(12)]
+
+    def refused(call, query, desc, backward, less):
+        need = query(C.byref(desc), backward)
+        assert need > less >= 0
+        desc.workspace = 1 << 30
+        for size in {0, less, need - 1}:
+            desc.workspace_bytes = size
+            assert call(C.byref(desc), None) == -1
+    scan = dict(x=a[0], x_row=8, gate=a[1], gate_row=8, y=a[2], y_row=8, B=2, D=8, type=1)
+    kept = N.GatedScanDesc(**scan, L=1000, states=a[3])
+    refused(lib.vmm_gated_scan, lib.vmm_gated_scan_workspace, N.GatedScanDesc(**scan, L=1000), 0, lib.vmm_gated_scan_workspace(C.byref(kept), 0))
+    refused(lib.vmm_gated_scan_bwd, lib.vmm_gated_scan_workspace, N.GatedScanDesc(**scan, L=1000, states=a[3]), 1, lib.vmm_gated_scan_workspace(C.byref(kept), 0))
+    ff = dict(x=a[0], ldx=40, w_gate=a[1], w_up=a[2], h=a[3], ldh=64, M=64, K=40, F=64, type=1)
+    bare = lib.vmm_gated_ff_workspace(C.byref(N.GatedFFDesc(M=64, K=40, F=64, type=1, ldx=40)), 0)  # nothing but sizes
+    for odd in (dict(x=a[0] + 2), dict(w_gate=a[1] + 2), dict(w_up=a[2] + 8), dict(ldx=41)):
+        refused(lib.vmm_gated_ff, lib.vmm_gated_ff_workspace, N.GatedFFDesc(**dict(ff, **odd)), 0, bare)
+    back = dict(ff, M=600, F=1024, g_pre=a[4], u_pre=a[5], dh=a[6], lddh=1024)
+    for wanted in (dict(dx=a[7], lddx=40), dict(dw_gate=a[8], dw_up=a[9])):
+        refused(lib.vmm_gated_ff_bwd, lib.vmm_gated_ff_workspace, N.GatedFFDesc(**back, **wanted), 1, lib.vmm_gated_ff_workspace(C.byref(N.GatedFFDesc(**back)), 1))

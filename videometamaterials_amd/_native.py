@@ -123,7 +123,7 @@ class GatedScanDesc(C.Structure):
         ("dx", c_ptr), ("dx_batch", c_i64), ("dx_row", c_i64),
         ("dgate", c_ptr), ("dgate_batch", c_i64), ("dgate_row", c_i64),
         ("dh_last", c_ptr), ("dh0", c_ptr),
-        ("workspace", c_ptr),
+        ("workspace", c_ptr), ("workspace_bytes", c_i64),
         ("L", c_i64),
         ("B", c_i32), ("D", c_i32), ("type", c_i32),
     ]
@@ -140,7 +140,7 @@ class GatedFFDesc(C.Structure):
         ("dh", c_ptr), ("lddh", c_i64),
         ("dx", c_ptr), ("lddx", c_i64),
         ("dw_gate", c_ptr), ("dw_up", c_ptr), ("db_gate", c_ptr), ("db_up", c_ptr),
-        ("workspace", c_ptr),
+        ("workspace", c_ptr), ("workspace_bytes", c_i64),
         ("M", c_i64),
         ("K", c_i32), ("F", c_i32), ("type", c_i32), ("act", c_i32),
     ]

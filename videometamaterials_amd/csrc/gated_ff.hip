@@ -552,6 +552,11 @@ Layout layout(const vmm_gated_ff_desc* d, bool backward) {
   return l;
 }
 
+bool room(const vmm_gated_ff_desc* d, bool backward) {
+  const long long bytes = layout(d, backward).bytes;
+  return bytes == 0 || (d->workspace && ((uintptr_t)d->workspace & 15) == 0 && d->workspace_bytes >= bytes);
+}
+
 template <int TYPE, bool ACOL, bool BCOL, bool GATED>
 int product(Gemm& q, const Shape& sh, int products, hipStream_t s) {
   const int r = sh.big ? 256 : 128;
@@ -675,7 +680,7 @@ extern "C" int vmm_gated_ff(const vmm_gated_ff_desc* d, vmm_stream_t stream) {
   if (bad_ff(d)) return -1;
   if (d->M == 0) return 0;
   if (!d->x || !d->w_gate || !d->w_up || !d->h || !d->g_pre != !d->u_pre) return -1;
-  if (layout(d, false).bytes > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15))) return -1;
+  if (!room(d, false)) return -1;
   hipStream_t s = (hipStream_t)stream;
   return d->type == 0 ? forward<0>(d, s) : d->type == 1 ? forward<1>(d, s) : forward<2>(d, s);
 }
@@ -684,7 +689,7 @@ extern "C" int vmm_gated_ff_bwd(const vmm_gated_ff_desc* d, vmm_stream_t stream)
   if (bad_ff(d)) return -1;
   if (!d->dw_gate != !d->dw_up) return -1;
   if (d->M > 0 && (!d->x || !d->w_gate || !d->w_up || !d->dh || !d->g_pre || !d->u_pre)) return -1;
-  if (layout(d, true).bytes > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15))) return -1;
+  if (!room(d, true)) return -1;
   hipStream_t s = (hipStream_t)stream;
   return d->type == 0 ? backward<0>(d, s) : d->type == 1 ? backward<1>(d, s) : backward<2>(d, s);
 }

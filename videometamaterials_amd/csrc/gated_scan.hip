@@ -643,7 +643,7 @@ int run(const ScanArgs& a, bool forward, hipStream_t s) {
 
 int scan(const vmm_gated_scan_desc* d, bool forward, hipStream_t s) {
   const Layout l = layout(d, !forward);
-  if (l.bytes > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15))) return -1;
+  if (l.bytes > 0 && (!d->workspace || ((uintptr_t)d->workspace & 15) || d->workspace_bytes < l.bytes)) return -1;
   ScanArgs a = {};
   a.d = *d;
   a.tiles = (d->D + CG * V - 1) / (CG * V);

@@ -101,6 +101,7 @@ Tensor workspace(int64_t (*query)(const D*, int32_t), D& d, bool backward, const
   if (size == 0) return {};
   Tensor w = at::empty({size}, like.options().dtype(at::kByte));
   d.workspace = w.data_ptr();
+  d.workspace_bytes = size;
   return w;
 }
 

@@ -1510,6 +1510,11 @@ class _Builder:
     # ---------------------------------------------------------------- load-history encoder of gated linear recurrences (Unet3D(cond_att_scan=True))
     SCAN_LAYERS = 3  # as many as the GRU encoder has (vddp.py:547)
 
+    def sequence_workspace(self, query, desc, backward: int) -> None:
+        """Room for one call, whose descriptor is complete but for it."""
+        desc.workspace_bytes = query(C.byref(desc), backward)
+        desc.workspace = self.ptr(self.alloc((desc.workspace_bytes + 3) // 4 + 4))
+
     def scan_encoder(self, cond_off: int) -> int:
         """Three layers over the (B, L) signal, one token per sample of it: x, gate = in_proj(s); y = scan(x, gate); s = y + down(silu(gate_proj(y)) * up_proj(y)).
         Returns the pointer of the last layer's rows [B][L][D]."""
@@ -1528,13 +1533,13 @@ class _Builder:
                                    L=Lg, B=B, D=D)
             if self.training:
                 scan.states = self.ptr(self.alloc(lib.vmm_gated_scan_states(C.byref(scan))))
-            scan.workspace = self.ptr(self.alloc((lib.vmm_gated_scan_workspace(C.byref(scan), 0) + 3) // 4 + 4))
+            self.sequence_workspace(lib.vmm_gated_scan_workspace, scan, 0)
             self.step(lib.vmm_gated_scan, (C.byref(scan),), f"sign_emb_scan layer {l}: scan")
             ff = N.GatedFFDesc(x=y, ldx=D, w_gate=self.wraw(pf + "gate_proj.weight"), w_up=self.wraw(pf + "up_proj.weight"), b_gate=self.wraw(pf + "gate_proj.bias"),
                                b_up=self.wraw(pf + "up_proj.bias"), h=h, ldh=F, M=B * Lg, K=D, F=F)
             if self.training:
                 ff.g_pre, ff.u_pre = self.ptr(self.alloc(B * Lg * F)), self.ptr(self.alloc(B * Lg * F))
-            ff.workspace = self.ptr(self.alloc((lib.vmm_gated_ff_workspace(C.byref(ff), 0) + 3) // 4 + 4))
+            self.sequence_workspace(lib.vmm_gated_ff_workspace, ff, 0)
             self.step(lib.vmm_gated_ff, (C.byref(ff),), f"sign_emb_scan layer {l}: gated feed-forward", flops=4.0 * B * Lg * D * F)
             self.dense_level([dict(x=h, w=self.wraw(pf + "down_proj.weight"), b=self.wraw(pf + "down_proj.bias"), add=y, ldadd=D, y=out, rows=B * Lg, K=F, N=D)],
                              f"sign_emb_scan layer {l}: back to the width, plus the states")
@@ -1559,13 +1564,13 @@ class _Builder:
             dy, dz = self.ptr(self.alloc(n)), self.ptr(self.alloc(2 * n))
             fb = N.GatedFFDesc(x=ff.x, ldx=D, w_gate=ff.w_gate, w_up=ff.w_up, g_pre=ff.g_pre, u_pre=ff.u_pre, dh=dh, lddh=F, dx=dy, lddx=D, dw_gate=pg(pf + "gate_proj.weight"),
                                dw_up=pg(pf + "up_proj.weight"), db_gate=pg(pf + "gate_proj.bias"), db_up=pg(pf + "up_proj.bias"), M=B * Lg, K=D, F=F)
-            fb.workspace = self.ptr(self.alloc((lib.vmm_gated_ff_workspace(C.byref(fb), 1) + 3) // 4 + 4))
+            self.sequence_workspace(lib.vmm_gated_ff_workspace, fb, 1)
             self.step(lib.vmm_gated_ff_bwd, (C.byref(fb),), f"sign_emb_scan layer {l}: gated feed-forward bwd", flops=8.0 * B * Lg * D * F)
             self.step(lib.vmm_lincomb, (dout, dy, None, 1.0, 1.0, 0.0, 0.0, dy, n), f"sign_emb_scan layer {l}: gradient of the states")
             sb = N.GatedScanDesc(x=scan.x, x_batch=scan.x_batch, x_row=scan.x_row, gate=scan.gate, gate_batch=scan.gate_batch, gate_row=scan.gate_row, states=scan.states,
                                  dy=dy, dy_batch=Lg * D, dy_row=D, dx=dz, dx_batch=Lg * 2 * D, dx_row=2 * D, dgate=dz + 4 * D, dgate_batch=Lg * 2 * D,
                                  dgate_row=2 * D, L=Lg, B=B, D=D)
-            sb.workspace = self.ptr(self.alloc((lib.vmm_gated_scan_workspace(C.byref(sb), 1) + 3) // 4 + 4))
+            self.sequence_workspace(lib.vmm_gated_scan_workspace, sb, 1)
             self.step(lib.vmm_gated_scan_bwd, (C.byref(sb),), f"sign_emb_scan layer {l}: scan bwd")
             dx = self.scratch(B * Lg * s["in_dim"]) if l > 0 else 0
             self.dense_bwd_level([dict(x=s["x"], w=self.wraw(pf + "in_proj.weight"), dy=dz, dx=dx, dw=self.pg(pf + "in_proj.weight"), db=self.pg(pf + "in_proj.bias"),
