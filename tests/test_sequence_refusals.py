@@ -91,3 +91,16 @@ def test_a_workspace_that_is_too_small_is_refused():
     back = dict(ff, M=600, F=1024, g_pre=a[4], u_pre=a[5], dh=a[6], lddh=1024)
     for wanted in (dict(dx=a[7], lddx=40), dict(dw_gate=a[8], dw_up=a[9])):
         refused(lib.vmm_gated_ff_bwd, lib.vmm_gated_ff_workspace, N.GatedFFDesc(**back, **wanted), 1, lib.vmm_gated_ff_workspace(C.byref(N.GatedFFDesc(**back)), 1))
+
+
+@pytest.mark.parametrize("name", ["ldx", "ldh", "lddh", "lddx"])
+@pytest.mark.parametrize("value", [-1, -8, 1 << 22])
+def test_leading_dimensions_of_the_feed_forward_product(name, value):
+    """A negative one would be read in front of its buffer."""
+    from videometamaterials_amd import _native as N
+    lib = N.lib()
+    a = [(k + 1) << 24 for k in range(12)]
+    d = N.GatedFFDesc(**dict(x=a[0], ldx=8, w_gate=a[1], w_up=a[2], h=a[3], ldh=8, g_pre=a[4], u_pre=a[5], dh=a[6], lddh=8, dx=a[7], lddx=8, M=4, K=8, F=8, type=1,
+                             workspace=1 << 30, workspace_bytes=1 << 30) | {name: value})
+    assert lib.vmm_gated_ff_workspace(C.byref(d), 0) == -1 and lib.vmm_gated_ff_workspace(C.byref(d), 1) == -1
+    assert lib.vmm_gated_ff(C.byref(d), None) == -1 and lib.vmm_gated_ff_bwd(C.byref(d), None) == -1

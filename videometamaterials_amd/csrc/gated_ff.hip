@@ -485,7 +485,7 @@ bool bad_ld(int64_t ld) { return ld < 0 || ld >= (1 << 22); }
 bool bad_ff(const vmm_gated_ff_desc* d) {
   // (K, F < 2^22: a tile of 256 rows is addressed with 32-bit byte offsets)
   if (!d || d->M < 0 || d->K < 1 || d->F < 1 || d->K >= (1 << 22) || d->F >= (1 << 22) || d->M >= (1LL << 31) || d->type < 0 || d->type > 2 || d->act < 0 ||
-      d->act > 1 || bad_ld(d->ldx) || bad_ld(d->ldh) || bad_ld(d->lddx))
+      d->act > 1 || bad_ld(d->ldx) || bad_ld(d->ldh) || bad_ld(d->lddh) || bad_ld(d->lddx))
     return true;
   const auto too_many = [](long long rows, long long cols) { return cdiv64(rows, 256) * cdiv64(cols, 256) >= (1LL << 23) - 8; };  // a launch has less than 2^32 threads
   return too_many(d->M, 2LL * d->F) || too_many(d->M, d->K) || too_many(d->F, d->K);
