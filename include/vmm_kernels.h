@@ -796,6 +796,7 @@ int vmm_gated_scan_bwd(const vmm_gated_scan_desc* d, vmm_stream_t stream);
  * Training: the forward leaves g = x Wg^T + bg and u = x Wu^T + bu in fp32, [M][F] each (g_pre, u_pre; both NULL: not kept).  Backward from dh:
  *   du = dh act(g), dg = dh u act'(g) (rounded to `type`: they are the operands of the products below),
  *   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dbg, dbu = column sums.   dx, (dWg, dWu), (dbg, dbu): each pair may be NULL; they are WRITTEN.
+ * Without rows (M = 0) nothing is read and the inputs may be NULL: the backward writes zeros to the gradients that are not empty.
  * workspace: vmm_gated_ff_workspace bytes, 16-byte aligned, contents irrelevant, for one call at a time; NULL where that is 0.
  * Refused (-1, by the query too): M of 2^31 and more, K, F, ldx, ldh, lddh, lddx of 2^22 and more or below zero, and 2^23 tiles of 256 x 256 in a product. */
 int64_t vmm_gated_ff_workspace(const vmm_gated_ff_desc* d, int32_t backward);

@@ -151,3 +151,21 @@ def test_strides_of_dimensions_of_one(gpu, dtype):
             h = gated_feed_forward(*leaves)
             out.append((h, *torch.autograd.grad(h, leaves, change(dh))))
         assert all(torch.equal(a, b) for a, b in zip(*out)), (M, K, F)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K,F", [(7, 9), (8, 16), (40, 300)])
+def test_ff_backward_without_rows_reads_nothing(gpu, dtype, K, F):
+    """Through the C ABI: no rows, none of the inputs there, and the gradients of the weights are zero."""
+    import ctypes as C
+    from videometamaterials_amd import _native as N
+    lib = N.lib()
+    dw, db = torch.full((2, F, K), 7.0, device=gpu, dtype=dtype), torch.full((2, F), 7.0, device=gpu, dtype=dtype)
+    d = N.GatedFFDesc(ldx=K, lddh=F, lddx=K, dw_gate=dw[0].data_ptr(), dw_up=dw[1].data_ptr(), db_gate=db[0].data_ptr(), db_up=db[1].data_ptr(), M=0, K=K, F=F,
+                      type=TYPES.index(dtype))
+    d.workspace_bytes = lib.vmm_gated_ff_workspace(C.byref(d), 1)
+    room = torch.empty(max(d.workspace_bytes, 16), dtype=torch.uint8, device=gpu)
+    d.workspace = room.data_ptr()
+    N.check(lib.vmm_gated_ff_bwd(C.byref(d), torch.cuda.current_stream().cuda_stream), "backward")
+    torch.cuda.synchronize()
+    assert not dw.any() and not db.any()

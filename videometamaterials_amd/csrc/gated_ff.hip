@@ -638,8 +638,10 @@ int backward(const vmm_gated_ff_desc* d, hipStream_t s) {
     VMM_LAUNCH_CHECK();
   }
   if (!(d->dx && d->M > 0) && !d->dw_gate) return 0;
-  Operands o;
-  if (const int e = operands<TYPE>(d, l, o, s)) return e;
+  Operands o = {};
+  if (d->M > 0) {  // (without rows nothing is read, neither x nor weights need be there, and the weights' gradients are zero)
+    if (const int e = operands<TYPE>(d, l, o, s)) return e;
+  }
   const long long plane = d->M * l.fp;
   if (d->dx && d->M > 0) {
     Gemm q = {};
