@@ -169,3 +169,11 @@ def test_ff_backward_without_rows_reads_nothing(gpu, dtype, K, F):
     N.check(lib.vmm_gated_ff_bwd(C.byref(d), torch.cuda.current_stream().cuda_stream), "backward")
     torch.cuda.synchronize()
     assert not dw.any() and not db.any()
+
+
+def test_smallest_bound_clips(gpu):
+    """The smallest positive float32 is a bound like any other: values that it leaves are below it."""
+    from videometamaterials_amd import clip_grad_norm_
+    g = normal(gpu, 4)(5000)
+    norm = clip_grad_norm_([g], 2.0 ** -149)
+    assert float(norm) > 60 and not g.any()

@@ -104,3 +104,14 @@ def test_leading_dimensions_of_the_feed_forward_product(name, value):
                              workspace=1 << 30, workspace_bytes=1 << 30) | {name: value})
     assert lib.vmm_gated_ff_workspace(C.byref(d), 0) == -1 and lib.vmm_gated_ff_workspace(C.byref(d), 1) == -1
     assert lib.vmm_gated_ff(C.byref(d), None) == -1 and lib.vmm_gated_ff_bwd(C.byref(d), None) == -1
+
+
+@pytest.mark.parametrize("bound", [0.0, -1.0, float("nan"), 1e-46, 2.0 ** -151])
+def test_bounds_that_are_no_positive_float32(bound):
+    """2^-151 becomes zero in float32, and zero means that nothing is clipped."""
+    import videometamaterials_amd as vm
+    from videometamaterials_amd.dp import DataParallelTrainer
+    for call in (lambda: vm.clip_grad_norm_([], bound), lambda: vm.ClippedAdam([torch.zeros(3)], max_norm=bound), lambda: DataParallelTrainer(None, max_grad_norm=bound)):
+        with pytest.raises(ValueError, match="positive"):
+            call()
+    assert float(vm.clip_grad_norm_([], 2.0 ** -149)) == 0.0

@@ -24,6 +24,7 @@ import os
 
 from . import _native as N
 from . import hostmath
+from .optim import positive_bound
 from .plan import _stream
 
 
@@ -341,8 +342,8 @@ class DataParallelTrainer:
         include/vmm_dp.h (its own RCCL communicator and side stream; also at world 1).  Default: $VMM_DP_ENGINE or "torch".
         max_grad_norm: the global norm that gradients are clipped to (None: no clipping) -- of the all-reduced, averaged and unscaled gradient, so every rank
         takes the same factor; the optimizer launch applies it.  The norm of the last step is then `self.grad_norm` (a device scalar)."""
-        if max_grad_norm is not None and not max_grad_norm > 0.0:
-            raise ValueError(f"max_grad_norm must be positive or None, got {max_grad_norm}")
+        if max_grad_norm is not None:
+            max_grad_norm = positive_bound(max_grad_norm, "max_grad_norm")
         self.max_grad_norm = max_grad_norm
         self.grad_norm: Optional[torch.Tensor] = None
         self.model = diffusion

@@ -6,11 +6,20 @@ over the gradients -- or ``DataParallelTrainer(max_grad_norm=...)``.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import Iterable, Optional
 
 import torch
 
 from . import _native as N
+
+
+def positive_bound(max_norm: float, what: str) -> float:
+    """`max_norm`, if it is positive as the float32 that it becomes: below half of the smallest one it would turn into zero, which means no clipping."""
+    max_norm = float(max_norm)
+    if not C.c_float(max_norm).value > 0.0:
+        raise ValueError(f"{what} must be positive (in float32), got {max_norm}")
+    return max_norm
 
 
 def _as_list(tensors, what: str) -> list:
@@ -31,9 +40,7 @@ def clip_grad_norm_(grads: Iterable[torch.Tensor], max_norm: float) -> torch.Ten
     """Scales `grads` (the gradient tensors themselves) in place by min(1, max_norm / (norm + 1e-6)) and returns the norm they had, as a float32 scalar on
     their device -- torch.nn.utils.clip_grad_norm_ without its host work; nothing is read or written a second time where the norm is within the bound.
     A NaN norm makes every gradient NaN, an infinite one makes the finite ones zero, as there.  Tensors must not overlap."""
-    max_norm = float(max_norm)
-    if not max_norm > 0.0:
-        raise ValueError(f"clip_grad_norm_: max_norm must be positive, got {max_norm}")
+    max_norm = positive_bound(max_norm, "clip_grad_norm_: max_norm")
     return N.binding().clip_grad_norm([grads] if isinstance(grads, torch.Tensor) else grads, max_norm)
 
 
@@ -48,8 +55,8 @@ class ClippedAdam:
         self.params = _as_list(params, "ClippedAdam")
         if not self.params:
             raise ValueError("ClippedAdam: no parameters")
-        if max_norm is not None and not max_norm > 0.0:
-            raise ValueError(f"ClippedAdam: max_norm must be positive or None, got {max_norm}")
+        if max_norm is not None:
+            max_norm = positive_bound(max_norm, "ClippedAdam: max_norm")
         if not (lr >= 0.0 and eps >= 0.0 and all(0.0 <= b < 1.0 for b in betas) and len(betas) == 2 and step >= 0):
             raise ValueError(f"ClippedAdam: lr {lr}, betas {betas}, eps {eps}, step {step}")
         self.lr, self.betas, self.eps, self.max_norm, self.steps_taken = lr, tuple(betas), eps, max_norm, int(step)
