@@ -177,3 +177,47 @@ def test_smallest_bound_clips(gpu):
     g = normal(gpu, 4)(5000)
     norm = clip_grad_norm_([g], 2.0 ** -149)
     assert float(norm) > 60 and not g.any()
+
+
+def test_captured_backward_beside_an_eager_graph_of_the_same_leaves(gpu):
+    """Refused while the eager graph lives; captured and replayed once it is gone."""
+    from videometamaterials_amd import gated_feed_forward, gated_linear_scan
+    from videometamaterials_amd._native import NativeError
+    n = normal(gpu, 5)
+    x, gate, w, v = n(2, 70, 16), n(2, 70, 16), n(24, 16), n(24, 16)
+    leaves = [t.requires_grad_() for t in (x, gate, w, v)]
+    dy = n(2, 70, 16)
+    dh = n(2, 70, 24)
+    scan = lambda: torch.autograd.grad(gated_linear_scan(x, gate)[0], (x, gate), dy)  # noqa: E731
+    product = lambda: torch.autograd.grad(gated_feed_forward(x, w, v), (x, w, v), dh)  # noqa: E731
+    side, scratch = torch.cuda.Stream(gpu), torch.zeros(4, device=gpu)
+    behind = lambda: torch.autograd.grad(gated_linear_scan(2 * x[:, ::1], gate.detach())[0], (x,), dy)  # noqa: E731  (torch's own operations in between)
+    for run, forward in ((scan, lambda: gated_linear_scan(x, gate)[0]), (product, lambda: gated_feed_forward(x, w, v)),
+                         (behind, lambda: gated_linear_scan(x, gate.detach())[0])):
+        alive = forward()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            scratch.add_(1.0)
+            with pytest.raises((NativeError, RuntimeError), match="eager graph"):
+                run()
+        want = torch.autograd.grad(alive, [t for t in leaves if t is not None], torch.ones_like(alive), allow_unused=True)
+        assert any(d is not None and bool(torch.isfinite(d).all()) for d in want)
+        del alive, want
+        if run is product:  # what an eager graph holds and nobody asks a gradient of does not matter
+            alive = gated_feed_forward(x.detach(), w, v.detach())
+            run = lambda: torch.autograd.grad(gated_feed_forward(x, w, v), (x, v), dh)  # noqa: E731
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        for seed in range(3):
+            with torch.no_grad():
+                for t in leaves:
+                    t.copy_(normal(gpu, 50 + seed)(*t.shape))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, run()))
+            torch.cuda.synchronize()

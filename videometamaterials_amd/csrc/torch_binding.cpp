@@ -3,13 +3,17 @@
 // A call of these operators on one token or a short signal is a few microseconds of kernels.  Written in Python over ctypes, descriptor, checks and
 // workspace took 14 to 20 us, an autograd function 50 to 80 more (its backward waits for the interpreter on another thread), and the tables of a norm over 367
 // tensors 126 us.  So this layer is compiled; what it calls is the C ABI, whose addresses `bind` is given from the library that is already loaded.
+#include <unordered_set>
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/autograd/graph_task.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include "../../include/vmm_kernels.h"
 
@@ -114,6 +118,32 @@ variable_list once(variable_list grads, const char* what) {
   return torch::autograd::DelayedError(c10::str(what, ": trying to differentiate twice a function that is differentiable once"), n).apply(std::move(grads));
 }
 
+// A leaf hands its gradient over on the stream that its first graph was made on.  Where an eager graph of that leaf is still alive, made on the default stream, a captured
+// backward would have to wait across to that stream, which no capture allows: it would end in the middle, and the process with it.
+void need_capturable(const char* what) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto* const wanted = torch::autograd::get_current_graph_task_exec_info();  // (empty: everything is)
+  std::vector<torch::autograd::Node*> next;
+  std::unordered_set<torch::autograd::Node*> seen;
+  const auto follow = [&](torch::autograd::Node& node) {
+    for (const auto& edge : node.next_edges()) {
+      if (!edge.function || !seen.insert(edge.function.get()).second) continue;
+      if (wanted && !wanted->empty())
+        if (const auto it = wanted->find(edge.function.get()); it == wanted->end() || !it->second.should_execute()) continue;
+      next.push_back(edge.function.get());
+    }
+  };
+  if (const auto node = torch::autograd::get_current_node()) follow(*node);
+  while (!next.empty()) {
+    torch::autograd::Node& node = *next.back();
+    next.pop_back();
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(&node))
+      if (const auto stream = node.stream(); stream && stream->id() == 0)
+        fail<NativeFault>(what, ": a captured backward needs leaves that no eager graph on the default stream holds: release that graph first");
+    follow(node);
+  }
+}
+
 // ---- gated linear recurrence
 
 const char* const SCAN = "gated_linear_scan";
@@ -170,6 +200,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(x.device());
+      need_capturable(SCAN);
       const Tensor dy = grads[0].defined() ? rows_of(grads[0]) : Tensor(), dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
       if (ctx->needs_input_grad(0)) dx = same(x.sizes(), x);
       if (ctx->needs_input_grad(1)) dgate = same(x.sizes(), x);
@@ -276,6 +307,7 @@ struct GatedFF : torch::autograd::Function<GatedFF> {
     {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(x.device());
+      need_capturable(FF);
       const Tensor dh = rows_of(grads[0]);
       if (ctx->needs_input_grad(0)) dx = same(x.sizes(), x);
       if (need_wg || need_wu) dwg = same(wg.sizes(), x), dwu = same(wg.sizes(), x);

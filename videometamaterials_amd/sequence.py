@@ -3,7 +3,8 @@ gradients.  They stand beside the GRU of ``cond_att_GRU`` (vddp.py:546-549): a r
 channels behind it; ``Unet3D(cond_att_scan=True)`` builds its load-history encoder from them.
 Checks, workspaces, launches and the autograd nodes are compiled (csrc/torch_binding.cpp).  Gradients are those of the backward pass; forward-mode derivatives,
 the transforms of torch.func, tracing (torch.jit.trace, make_fx, torch.export) and tensors that stand in for others are refused (NotImplementedError); torch.compile
-breaks its graph around a call.
+breaks its graph around a call.  Calls and their backward passes may be captured into a HIP graph; a captured backward whose leaves an eager graph on the default stream
+still holds is refused (the capture would end the process).
 """
 from __future__ import annotations
 
