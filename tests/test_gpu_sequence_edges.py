@@ -221,3 +221,27 @@ def test_captured_backward_beside_an_eager_graph_of_the_same_leaves(gpu):
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, run()))
             torch.cuda.synchronize()
+
+
+def test_ff_products_of_fp32_values(gpu):
+    """Single products (K = 1) of values whose parts are as large as parts get.  With wg = 64 the gate's pre-activation is 64 x without an error and silu passes it, so
+    h = 64 x (x wu): the product's parts that are left out are 2^-24 = U of it at most, the product with 64 x rounds by U.  The last sum adds the largest product to
+    a smaller accumulator, which the matrix unit then floors to the sum's last place (1 * 1 + 1.5 2^-24 gives 1, 1 * 1 - 2^-30 gives 1 - 2^-24; an accumulator
+    that is the larger is rounded to nearest): up to 2 U, always downwards; the sums before it lose 2^-7 of that each.
+    What is left out has no side, so the mean over 2^18 products is that of the floor alone, half a last place: between zero and -U (parts that are cut would add
+    0.63 U to it)."""
+    from videometamaterials_amd import gated_feed_forward
+    bits = torch.randint(0, 1 << 23, (4096,), generator=torch.Generator().manual_seed(1), dtype=torch.int32)
+    bits[:8] = torch.tensor([0x00ffff, 0x7fffff, 0x007fff, 0x008000, 0x7f7fff, 0x00ff7f, 0x7e8080, 0x7fff80])
+    value = (bits | 0x3f800000).view(torch.float32)
+    x, wu = value[:, None].to(gpu), value[:64, None].contiguous().to(gpu)
+    h = gated_feed_forward(x, torch.full_like(wu, 64.0), wu).double().cpu()
+    want = 64 * value.double()[:, None] ** 2 * value[:64].double()
+    off = (h - want) / want
+    assert float(off.abs().max()) <= (1 + 2 + 1 + 2.0 ** -5) * U
+    assert -1.05 * U < float(off.mean()) < 0.05 * U
+    # next to the largest value a part is not rounded up to infinity; an infinite operand gives NaN
+    top = torch.tensor([[torch.finfo(torch.float32).max], [-3.39e38], [float("inf")], [1.0]], device=gpu)
+    one = torch.tensor([[0.25]], device=gpu)
+    h = gated_feed_forward(top, torch.zeros_like(one), one)
+    assert not h[:2].any() and bool(torch.isnan(h[2]).all()) and not h[3].any()

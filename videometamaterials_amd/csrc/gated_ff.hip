@@ -8,8 +8,9 @@
 //   forward   A = x, B = rows of Wg and Wu side by side in one tile: a wave holds the same places of g and u, so activation and product need no exchange
 //   dx        A = dg, B = Wg (stored [k][j]), then the part of du and Wu
 //   dW        A = dg (stored [k][i]), B = x (stored [k][j]);  gate and up side by side in the grid
-// fp32 operands are split into three bf16 parts without a remainder (24 = 3 x 8 bits), and a product is the sum of the six parts that reach 2^-16 of it,
-// small ones first; what is left out is below 2^-22.  That is six matrix passes at 16 times the rate of fp32 ones.
+// fp32 operands are split into three bf16 parts without a remainder (24 = 3 x 8 bits), each rounded to nearest, so the second is below 2^-8 and the third below 2^-17
+// of the value's power of two; a product is the sum of the six products of parts that reach 2^-17 of it, small ones first.  What is left out, second times third
+// both ways, is below 2^-24 and of either sign (the matrix unit itself floors an accumulator that is smaller than a product to the sum's last place).  That is six matrix passes at 16 times the rate of fp32 ones.
 //
 // A tile step is 64 reduced indexes.  It goes from memory to LDS directly (buffer loads with an LDS destination: no registers, and what lies
 // outside the operand arrives as zero), into the one of two buffers that the matrix instructions do not read.  Such a load fills 1 KiB of LDS in lane order,
@@ -357,12 +358,14 @@ __global__ __launch_bounds__(256) void ff_join_gated_kernel(const Gemm q) {
 // ---- operands: three bf16 parts of fp32 values, or 16-bit values whose rows are not made of whole 16-byte pieces, laid out with padded rows
 struct Layin { const void* src[3]; u16* dst[3]; long long rows[3], ld[3]; int cols, pitch; };
 
+__device__ __forceinline__ unsigned near16(float x) { return (unsigned)__builtin_bit_cast(u16, (__bf16)x) << 16; }  // bits of the nearest bf16 as fp32
 __device__ __forceinline__ void thirds(float x, u16& h, u16& m, u16& l) {
-  const unsigned a = __float_as_uint(x) & 0xffff0000u;
+  unsigned a = near16(x);
+  if ((a & 0x7fffffffu) == 0x7f800000u) a = __float_as_uint(x) & 0xffff0000u;  // (a finite value next to the largest is cut: rounded up it would be infinite)
   const float r = x - __uint_as_float(a);
-  const unsigned b = __float_as_uint(r) & 0xffff0000u;
+  const unsigned b = near16(r);
   const float s = r - __uint_as_float(b);
-  h = a >> 16; m = b >> 16; l = __float_as_uint(s) >> 16;
+  h = a >> 16; m = b >> 16; l = near16(s) >> 16;
 }
 template <int TYPE>
 __device__ __forceinline__ void put(u16* p, long long plane, float v) {
