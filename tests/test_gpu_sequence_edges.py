@@ -245,3 +245,90 @@ def test_ff_products_of_fp32_values(gpu):
     one = torch.tensor([[0.25]], device=gpu)
     h = gated_feed_forward(top, torch.zeros_like(one), one)
     assert not h[:2].any() and bool(torch.isnan(h[2]).all()) and not h[3].any()
+
+
+def recurrence(f, b, h):
+    """h_t = f_t h_(t-1) + b_t over dimension 1 in 64 bits, in pieces that are walked side by side and then joined."""
+    B, L, D = f.shape
+    c = max(1, math.isqrt(L))
+    n = -(-L // c)
+    pad = n * c - L
+    f = torch.cat([f, torch.ones(B, pad, D, dtype=f.dtype)], 1).view(B, n, c, D)
+    b = torch.cat([b, torch.zeros(B, pad, D, dtype=b.dtype)], 1).view(B, n, c, D)
+    out, through = torch.empty_like(b), torch.empty_like(f)
+    p, q = torch.ones_like(f[:, :, 0]), torch.zeros_like(b[:, :, 0])
+    for t in range(c):
+        p, q = p * f[:, :, t], q * f[:, :, t] + b[:, :, t]
+        through[:, :, t], out[:, :, t] = p, q
+    for k in range(n):
+        out[:, k] += through[:, k] * h[:, None]
+        h = out[:, k, -1]
+    return out.view(B, n * c, D)[:, :L]
+
+
+def scan_with_bounds(x, gate, h0, dy, dlast):
+    """(name, value in 64 bits, sum of absolute values, bound) of y, last, dx, dgate, dh0.  The bound follows the decay of each channel: a gate that is open (f > i) is off by its
+    own rounding and by i / f times the (|g| + 6) U of i, a closed one by (|g| + 6) U, and a step rounds three times more (sum and map); a state's error is what the step before
+    hands on, E_t = f (E_(t-1) + 2 (rho + 3 U) H_(t-1)) + 2 (|g| + 8) U i |x|, with H the same recurrence of absolute values, and a factor of two for how maps are joined."""
+    x, g, h0, dy, dlast = (v.detach().double().cpu() for v in (x, gate, h0, dy, dlast))
+    f, i = torch.sigmoid(g), torch.sigmoid(-g)
+    rho, wide = 2 * U * (4 + torch.clamp(i / f, max=1.0) * (g.abs() + 6)), 2 * U * (g.abs() + 8)
+
+    def shifted(first, rest):
+        return torch.cat([first[:, None], rest[:, :-1]], 1)
+    h, H = recurrence(f, i * x, h0), recurrence(f, i * x.abs(), h0.abs())
+    E = recurrence(f, f * rho * shifted(h0.abs(), H) + wide * i * x.abs(), torch.zeros_like(h0))
+    before, Hb, Eb = shifted(h0, h), shifted(h0.abs(), H), shifted(torch.zeros_like(h0), E)
+
+    def back(b, c):  # c_t = f_t (b_t + c_(t+1)), from the end
+        return recurrence(f.flip(1), (f * b).flip(1), c).flip(1)
+
+    def after(c, last):  # what step t gets from behind it
+        return torch.cat([c[:, 1:], last[:, None]], 1)
+    c, C = back(dy, dlast), back(dy.abs(), dlast.abs())
+    dh, DH = dy + after(c, dlast), dy.abs() + after(C, dlast.abs())
+    Ec = recurrence(f.flip(1), (f * rho * DH).flip(1), torch.zeros_like(h0)).flip(1)
+    Ed = after(Ec, torch.zeros_like(h0)) + U * DH
+    yield "y", h, H, E
+    yield "last", h[:, -1], H[:, -1], E[:, -1]
+    yield "dx", dh * i, DH * i, i * (Ed + wide * DH)
+    yield "dgate", dh * (before - x) * f * i, DH * (Hb + x.abs()) * f * i, f * i * (Ed * (Hb + x.abs()) + DH * Eb + 2 * wide * DH * (Hb + x.abs()))
+    yield "dh0", c[:, 0], C[:, 0], Ec[:, 0]
+
+
+LONG = [(1, 800_000, 6), (1, 530_000, 4), (2, 20_011, 36), (2, 4_093, 101)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,L,D", LONG)
+def test_scan_long_memories(gpu, dtype, B, L, D):
+    """Sequences of thousands of steps and of more than 256 groups of 1024 (anchors), with memories of two steps to a million side by side: every output element by element,
+    and the same calls in pieces of an eighth (fewer than 256 groups, whole ones), the state handed on.  A piece has the same maps, joined in another order: a state differs by
+    one rounding for each of 16 units, 16 rows and 256 groups it comes through, twice."""
+    n = normal(gpu, L)
+    # a memory of e^lean steps; the state in front and its gradient are as large as what comes on the way
+    lean = torch.linspace(0.0, 14.0, D, device=gpu)[torch.randperm(D, generator=torch.Generator().manual_seed(D)).to(gpu)]
+    x, gate, h0 = n(B, L, D, dtype=dtype), (n(B, L, D, k=0.5) + lean).to(dtype), n(B, D)
+    dy, dlast = n(B, L, D, k=2e-3, dtype=dtype), n(B, D)
+    got = scan_all(x, gate, h0, dy, dlast)
+    sub = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -150}[dtype]
+    sizes = {}
+    for value, (what, want, size, bound) in zip(got, scan_with_bounds(x, gate, h0, dy, dlast)):
+        if value.dtype == dtype:
+            bound = bound * (1 + half_step(dtype)) + half_step(dtype) * want.abs() + sub
+        within(value, want, bound + 17 * 2.0 ** -150, what)
+        sizes[what] = size, want
+    from videometamaterials_amd import gated_linear_scan
+    leaves = [v.detach().requires_grad_() for v in (x, gate, h0)]
+    h, ys, piece = leaves[2], [], -(-L // 8 // 1024) * 1024
+    for t in range(0, L, piece):
+        y, h = gated_linear_scan(leaves[0][:, t:t + piece], leaves[1][:, t:t + piece], h)
+        ys.append(y)
+    pieces = (torch.cat(ys, 1).detach(), h.detach(), *torch.autograd.grad((torch.cat(ys, 1), h), leaves, (dy, dlast)))
+    joins = 2 * (16 + 16 + 256) * U
+    channel = lambda v: v.reshape(-1, D).norm(dim=0)  # noqa: E731
+    for value, other, (what, (size, want)) in zip(got, pieces, sizes.items()):
+        step = 2 * half_step(dtype) if value.dtype == dtype else 0.0
+        within(value, other.double().cpu(), 2 * joins * size + step * other.double().cpu().abs() + 2 * sub, what + " in pieces")
+        if value.dim() == 3:  # (this bound is small beside the results, in the longest memories too: an output of zeros would not pass)
+            assert bool((channel(2 * joins * size) < 0.2 * channel(want)).all()), (what, channel(2 * joins * size) / channel(want))
