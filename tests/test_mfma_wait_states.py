@@ -143,8 +143,49 @@ def test_results_of_matrix_instructions_are_waited_for(name, tmp_path):
         path.write_bytes(image)
         text = subprocess.run([os.path.join(LLVM, "llvm-objdump"), "-d", str(path)], check=True, capture_output=True, text=True).stdout
         for function, code in functions(text).items():
-            products += sum(op.startswith("v_mfma") for _, op, _, _ in code)
-            if code:
+            here = sum(op.startswith("v_mfma") for _, op, _, _ in code)
+            products += here
+            if here:
                 found += [f"{function}: {w} of {need} wait states from {a:#x} to {b:#x}" for w, need, a, b in too_early(code)]
     assert products > 1000
     assert not found, "\n".join(found[:40])
+
+
+def test_tiles_have_landed_at_every_barrier(tmp_path):
+    """The product kernel of the gated feed-forward fetches its tiles to LDS directly, and other waves read them behind the next barrier: on every way from such a load
+    to a barrier the wave has to wait for it (vmcnt(0)).  The barrier does not do that by itself."""
+    library = os.path.join(PACKAGE, "libvmm_hip.so")
+    if not os.path.exists(library) or not os.path.exists(os.path.join(LLVM, "llvm-objdump")):
+        pytest.skip("not built here, or no disassembler")
+    copy = shutil.copy(library, tmp_path / "l.so")
+    kernels = loads = 0
+    for n, image in enumerate(code_objects(str(copy))):
+        path = tmp_path / f"{n}.elf"
+        path.write_bytes(image)
+        if b"ff_gemm_kernel" not in image:
+            continue
+        text = subprocess.run([os.path.join(LLVM, "llvm-objdump"), "-d", str(path)], check=True, capture_output=True, text=True).stdout
+        for function, code in functions(text).items():
+            if "ff_gemm_kernel" not in function or not code:
+                continue
+            kernels += 1
+            index, start = {address: i for i, (address, _, _, _) in enumerate(code)}, code[0][0]
+            for i, (address, op, rest, _) in enumerate(code):
+                if not (op.startswith("buffer_load") and rest.endswith("lds")):
+                    continue
+                loads += 1
+                seen, ways = set(), [i + 1]
+                while ways:
+                    j = ways.pop()
+                    if j in seen or j >= len(code):
+                        continue
+                    seen.add(j)
+                    _, o, r, target = code[j]
+                    if o == "s_endpgm" or (o == "s_waitcnt" and "vmcnt(0)" in r):
+                        continue
+                    assert o != "s_barrier", f"{function}: {code[j][0]:#x} is reached with the load of {address:#x} under way"
+                    if o == "s_branch" or o.startswith("s_cbranch"):
+                        ways.append(index[start + target])
+                    if o != "s_branch":
+                        ways.append(j + 1)
+    assert kernels == 18 and loads > 18 * 8

@@ -80,7 +80,7 @@ __device__ __forceinline__ float exp_minus(float m) {
 // The activation's factor P (a = g P) and its derivative P + g P'.
 //   silu: P = sigmoid(g) from e^-|g|, P' = P (1 - P)
 //   gelu: P = Phi(g), the normal distribution: Phi(-|g|) = e^(-g^2/2) erfcx(|g| / sqrt 2) / 2, whose last two factors are a polynomial in
-//         t = 1 / (1 + |g| / sqrt 8), fitted for the least relative error over |g| <= 13.4 (4.2e-8; 3.2e-7 as evaluated); P' = e^(-g^2/2) / sqrt(2 pi)
+//         t = 1 / (1 + |g| / sqrt 8), fitted for the least relative error over |g| <= 13.4 (5.4e-8 with its coefficients in fp32; 3.2e-7 as evaluated); P' = e^(-g^2/2) / sqrt(2 pi)
 // (erff and the exact division took half of the epilogue: 512 x 256 x 128 values, 13 us a tile)
 template <int TYPE, int ACT, bool SLOPE>
 __device__ __forceinline__ float act_parts(float g, float& slope) {

@@ -6,8 +6,8 @@
 // All three are bound by memory: the norm reads every gradient once (4 or 2 bytes a value), clipping in place reads and writes it -- and does neither
 // where c = 1 --, the Adam step moves 28 bytes a value in fp32 and takes c from device memory, so that clipping costs it no pass of its own.
 //
-// Tensors come as a HOST array of jobs that travels in the kernel arguments (gradients move from step to step, and a table in device memory would need a
-// copy that a captured graph replays from stale host memory).  4 KiB of arguments hold NORM_JOBS / ADAM_JOBS tensors a launch.  The tensors of a launch
+// Tensors come as a HOST array of jobs that travels in the kernel arguments: gradients move from step to step, and a table in device memory would need a copy at
+// each (which a captured norm or clipping would replay from stale host memory; the optimizer step is not captured, and could do with one).  4 KiB of arguments hold NORM_JOBS / ADAM_JOBS tensors a launch.  The tensors of a launch
 // are laid end to end in chunks of CHUNK values; every workgroup takes an equal run of chunks, so one large matrix and hundreds of short vectors
 // balance alike, and the number of partial sums is bounded by the grid and not by the number of values.
 //

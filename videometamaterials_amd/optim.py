@@ -32,14 +32,14 @@ def _as_list(tensors, what: str) -> list:
 
 def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
     """sqrt of the sum of all squares of `grads` (any mixture of float32, bfloat16, float16), as a float32 scalar on their device; sums are held in 64 bits
-    and have the same bits every time.  No tensors: a zero on the CPU."""
+    and have the same bits every time.  Tensors must be contiguous.  No tensors: a zero on the CPU."""
     return N.binding().grad_norm([grads] if isinstance(grads, torch.Tensor) else grads)
 
 
 def clip_grad_norm_(grads: Iterable[torch.Tensor], max_norm: float) -> torch.Tensor:
     """Scales `grads` (the gradient tensors themselves) in place by min(1, max_norm / (norm + 1e-6)) and returns the norm they had, as a float32 scalar on
     their device -- torch.nn.utils.clip_grad_norm_ without its host work; nothing is read or written a second time where the norm is within the bound.
-    A NaN norm makes every gradient NaN, an infinite one makes the finite ones zero, as there.  Tensors must not overlap."""
+    A NaN norm makes every gradient NaN, an infinite one makes the finite ones zero, as there.  Tensors must be contiguous and not overlap."""
     max_norm = positive_bound(max_norm, "clip_grad_norm_: max_norm")
     return N.binding().clip_grad_norm([grads] if isinstance(grads, torch.Tensor) else grads, max_norm)
 
