@@ -12,7 +12,7 @@
 // that step 2 goes through 255 groups at the most.  Which maps are joined in which order depends on the sizes alone: the same bits every time.
 //
 // What bounds it: memory and instructions alike.  3 values a step move forward and 5 backward, plus 2 for the maps, which the third step finds in the 256 MB
-// of last-level cache for the most part: it walks time from the end, where step 1 has read last.  65536 steps of 1024 channels in bf16 take 56 + 8 + 69 us: the
+// of last-level cache for the most part: it walks time from the end, where step 1 has read last.  65536 steps of 1024 channels in bf16 take 57 + 8 + 70 us: the
 // maps read at a copy's 4.8 TB/s; the 402 MB that have to move once are 83 us of it.  Each value costs some thirty instructions, so whatever can be
 // decided for a whole unit is (see `unit`).  Passing states from workgroup to workgroup inside one launch would read all of it once, and was
 // built first; workgroups then poll each other's results past the caches, and the same took 192 us (228 us with groups and tiles of 128 steps; 370 us with tiles of 64).
@@ -177,9 +177,9 @@ __device__ __forceinline__ void wave_join(float* p, float* q, float* pe, float* 
 }
 
 // Consecutive workgroups go to different XCDs.  Where rows do not start on cache lines, each XCD gets a run of the work instead, so that tiles beside each
-// other share the lines at their borders in one L2: 4093 steps of 8 x 1000 channels in bf16 take 26 / 33 / 27 / 68 us for forward maps and application,
-// backward maps and application where the plain order takes 33 / 47 / 33 / 86; rows that do (65536 x 1024) 56 / 69 us in the plain order and
-// 60 / 70 in runs.  The grid is eight runs; numbers from `work` on are nobody's.
+// other share the lines at their borders in one L2: 4093 steps of 8 x 1000 channels in bf16 take 27 / 35 / 27 / 68 us for forward maps and application,
+// backward maps and application where the plain order takes 34 / 48 / 33 / 86; rows that do (65536 x 1024) 57 / 70 us in the plain order and
+// 61 / 71 in runs.  The grid is eight runs; numbers from `work` on are nobody's.
 __device__ __forceinline__ unsigned number(const ScanArgs& a, unsigned work) {
   return a.runs ? (blockIdx.x & 7) * ((work + 7) / 8) + (blockIdx.x >> 3) : blockIdx.x;
 }
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(1024) void scan_map_kernel(const ScanArgs a) {
     }
   };
   // Nearly every group is whole (all steps within the length, all channels there), and works without masks, paddings and their moves: 85 -> 69 us for the
-  // application and 59 -> 56 for the maps of 65536 x 1024.  (A third form, for units behind a sequence's end, gained nothing.)
+  // application and 59 -> 56 for the maps of 65536 x 1024 (with closed gates exact, 70 and 57).  (A third form, for units behind a sequence's end, gained nothing.)
   if (columns >= CG * V && (group + 1) * GROUP <= a.units && len >= (BACK ? a.units - group * GROUP : (group + 1) * GROUP) * (long long)UNIT && has_x) unit(std::true_type{});
   else unit(std::false_type{});
 }
