@@ -332,3 +332,26 @@ def test_scan_long_memories(gpu, dtype, B, L, D):
         within(value, other.double().cpu(), 2 * joins * size + step * other.double().cpu().abs() + 2 * sub, what + " in pieces")
         if value.dim() == 3:  # (this bound is small beside the results, in the longest memories too: an output of zeros would not pass)
             assert bool((channel(2 * joins * size) < 0.2 * channel(want)).all()), (what, channel(2 * joins * size) / channel(want))
+
+
+def test_gradients_that_are_lazily_negated(gpu):
+    """The imaginary part of a conjugated tensor is its negative in memory, whatever its strides."""
+    from videometamaterials_amd import gated_feed_forward, gated_linear_scan
+    n = normal(gpu, 9)
+
+    def negated(*shape):
+        t = torch.complex(n(*shape), n(*shape)).conj().imag
+        assert t.is_neg()
+        return t
+    for B, L, D in ((2, 70, 1), (1, 1, 1), (2, 70, 12)):
+        x, gate = n(B, L, D).requires_grad_(), n(B, L, D).requires_grad_()
+        y, last = gated_linear_scan(x, gate)
+        dy, dlast = negated(B, L, D), negated(B, D)
+        got = torch.autograd.grad((y, last), (x, gate), (dy, dlast), retain_graph=True)
+        want = torch.autograd.grad((y, last), (x, gate), (dy.resolve_neg().contiguous(), dlast.resolve_neg().contiguous()))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        w, v = n(D, D).requires_grad_(), n(D, D)
+        h = gated_feed_forward(x, w, v)
+        dh = negated(B, L, D)
+        got = torch.autograd.grad(h, (x, w), dh, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(h, (x, w), dh.resolve_neg().contiguous())))

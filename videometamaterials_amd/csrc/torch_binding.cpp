@@ -88,6 +88,8 @@ std::string shape(const Tensor& t) { return c10::str(t.sizes()); }
 Tensor rows_of(const Tensor& t) {
   return (t.stride(-1) == 1 || t.size(-1) <= 1) && (t.stride(-2) < (1 << 22) || t.size(-2) <= 1) ? t : t.contiguous();
 }
+// a gradient as its values are in memory (part of a conjugated complex one can come negated, to be)
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 int64_t row_stride(const Tensor& t) { return t.size(-2) > 1 ? t.stride(-2) : t.size(-1); }
 
 template <typename T>
@@ -201,7 +203,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(x.device());
       need_capturable(SCAN);
-      const Tensor dy = grads[0].defined() ? rows_of(grads[0]) : Tensor(), dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+      const Tensor dy = grads[0].defined() ? rows_of(plain(grads[0])) : Tensor(), dlast = grads[1].defined() ? plain(grads[1]).contiguous() : Tensor();
       if (ctx->needs_input_grad(0)) dx = same(x.sizes(), x);
       if (ctx->needs_input_grad(1)) dgate = same(x.sizes(), x);
       if (ctx->saved_data["state"].toBool() && ctx->needs_input_grad(2)) dh0 = fp32({x.size(0), x.size(2)}, x);
@@ -308,7 +310,7 @@ struct GatedFF : torch::autograd::Function<GatedFF> {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(x.device());
       need_capturable(FF);
-      const Tensor dh = rows_of(grads[0]);
+      const Tensor dh = rows_of(plain(grads[0]));
       if (ctx->needs_input_grad(0)) dx = same(x.sizes(), x);
       if (need_wg || need_wu) dwg = same(wg.sizes(), x), dwu = same(wg.sizes(), x);
       if (need_bg) dbg = same({wg.size(0)}, x);
