@@ -792,7 +792,8 @@ int vmm_gated_scan_bwd(const vmm_gated_scan_desc* d, vmm_stream_t stream);
 
 /* ---- gated feed-forward product: h = act(x Wg^T + bg) * (x Wu^T + bu), both projections, the activation and the product in one kernel.
  * x [M][K] (row stride ldx), Wg, Wu [F][K] and the biases [F] (NULL: none), h [M][F] (ldh), all of `type`; act 0 silu, 1 gelu (erf).
- * fp32: every product of two fp32 values is made of six products of their bf16 thirds and is exact to 2^-24, to either side; an infinite operand gives NaN, not infinity.
+ * fp32: every product of two fp32 values is made of six products of their bf16 thirds and is exact to 2^-24, to either side; an infinite operand gives NaN, not infinity,
+ * and one below 2^-110 is as good as a multiple of 2^-133 (the smallest bf16 number, of which its last third would be a fraction).
  * Training: the forward leaves g = x Wg^T + bg and u = x Wu^T + bu in fp32, [M][F] each (g_pre, u_pre; both NULL: not kept).  Backward from dh:
  *   du = dh act(g), dg = dh u act'(g) (rounded to `type`: they are the operands of the products below),
  *   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dbg, dbu = column sums.   dx, (dWg, dWu), (dbg, dbu): each pair may be NULL; they are WRITTEN.

@@ -10,7 +10,8 @@
 //   dW        A = dg (stored [k][i]), B = x (stored [k][j]);  gate and up side by side in the grid
 // fp32 operands are split into three bf16 parts without a remainder (24 = 3 x 8 bits), each rounded to nearest, so the second is below 2^-8 and the third below 2^-17
 // of the value's power of two; a product is the sum of the six products of parts that reach 2^-17 of it, small ones first.  What is left out, second times third
-// both ways, is below 2^-24 and of either sign (the matrix unit itself floors an accumulator that is smaller than a product to the sum's last place).  That is six matrix passes at 16 times the rate of fp32 ones.
+// both ways, is below 2^-24 and of either sign (the matrix unit itself floors an accumulator that is smaller than a product to the sum's last place).
+// The last bit of a value from 2^-110 on is 2^-133 at the least, the smallest bf16 number; smaller values are rounded to a multiple of it.  That is six matrix passes at 16 times the rate of fp32 ones.
 //
 // A tile step is 64 reduced indexes.  It goes from memory to LDS directly (buffer loads with an LDS destination: no registers, and what lies
 // outside the operand arrives as zero), into the one of two buffers that the matrix instructions do not read.  Such a load fills 1 KiB of LDS in lane order,

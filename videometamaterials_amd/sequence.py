@@ -35,7 +35,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
 
     w_gate, w_up (F, K) and the biases (F,) (both or none) as torch.nn.Linear keeps them; activation "silu" or "gelu" (the erf form); everything float32,
     bfloat16 or float16 alike.  Sums are held in float32 for every type; the float32 products are made on the matrix cores from three bfloat16 parts of
-    each value, to float32's own accuracy (an infinite operand gives NaN).  Differentiable (once) in every tensor; the backward's dg and du are
+    each value, to float32's own accuracy (an infinite operand gives NaN; an operand below 2^-110 is rounded to a multiple of 2^-133, bfloat16's smallest number).  Differentiable (once) in every tensor; the backward's dg and du are
     rounded to the type: 16-bit gradients of x and the weights are off by that rounding and their own (1.41 times their own alone), and with float16 the
     loss has to be scaled as for any float16 product."""
     act = ACTIVATIONS.get(activation)
