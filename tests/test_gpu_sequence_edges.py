@@ -373,3 +373,28 @@ def test_ff_range_of_fp32_operands(gpu):
             assert torch.equal(got, v.double()), e
         else:
             assert float((got - v.double()).abs().max()) <= 2.0 ** -134, e
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("L", [50, 200, 3000])
+def test_scan_gradients_of_extreme_gates(gpu, dtype, L):
+    """Gates of 200, infinity and the type's largest value, both signs: all or nothing, and no gradient of their own.  A NaN gate reaches what comes behind it forwards and what
+    lies before it backwards, and nothing else."""
+    n = normal(gpu, 12)
+    x, gate, h0, dy, dlast = n(1, L, 8, dtype=dtype), n(1, L, 8, dtype=dtype), n(1, 8), n(1, L, 8, dtype=dtype), n(1, 8)
+    top = torch.finfo(dtype).max
+    for d, g in enumerate((200.0, -200.0, math.inf, -math.inf, top, -top)):
+        gate[..., d] = g
+    at = L // 2
+    gate[0, at, 7] = math.nan
+    y, last, dx, dgate, dh0 = (v.double().cpu() for v in scan_all(x, gate, h0, dy, dlast))
+    h, dh, dl = h0.double().cpu()[0], dy.double().cpu()[0], dlast.double().cpu()[0]
+    for d in (0, 2, 4):  # the state stands: its gradient is the sum of all that is asked of it, 64 bits of which the sum of L rounded steps knows (L + 8) U
+        assert torch.equal(y[0, :, d], h[d].float().to(dtype).double().expand(L)) and not dx[0, :, d].any() and not dgate[0, :, d].any()
+        assert abs(float(dh0[0, d] - dh[:, d].sum() - dl[d])) <= (L + 8) * U * float(dh[:, d].abs().sum() + dl[d].abs())
+    for d in (1, 3, 5):  # every step is its own input
+        assert torch.equal(y[0, :, d], x.double().cpu()[0, :, d]) and not dgate[0, :, d].any() and float(dh0[0, d]) == 0.0
+        assert torch.equal(dx[0, :-1, d], dh[:-1, d]) and torch.equal(dx[0, -1, d], (dh[-1, d] + dl[d]).float().to(dtype).double())
+    assert bool(torch.isfinite(y[0, :at, 7]).all()) and bool(torch.isnan(y[0, at:, 7]).all()) and bool(torch.isnan(last[0, 7]))
+    assert bool(torch.isnan(dx[0, :at, 7]).all()) and bool(torch.isfinite(dx[0, at + 1:, 7]).all()) and bool(torch.isnan(dh0[0, 7]))
+    assert all(bool(torch.isfinite(v[..., 6]).all()) for v in (y, last, dx, dgate, dh0))
